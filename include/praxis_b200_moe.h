@@ -45,6 +45,10 @@ enum {
 
 enum { PRAXIS_B200_SIGMOID = 0, PRAXIS_B200_SOFTMAX = 1 };
 
+/* How praxis_b200_route_groups judges a group of experts: by the sum of its
+ * two best biased scores, or by its best one. */
+enum { PRAXIS_B200_GROUP_TOP2 = 0, PRAXIS_B200_GROUP_MAX = 1 };
+
 /* Grouped-GEMM epilogues (praxis_b200_grouped_gemm). */
 enum {
   PRAXIS_B200_EPI_PLAIN = 0,   /* out = bf16(acc) */
@@ -92,6 +96,18 @@ int praxis_b200_router_logits(const void* x, const void* weight, int32_t weight_
  * praxis/kernels/router_fused.py:738-804 (route_dispatch). E <= 256, k <= 8. */
 int praxis_b200_route(const float* logits, const float* bias, int64_t tokens, int32_t experts, int32_t top_k,
                       int32_t activation, int64_t* top_idx, void* gate, int device, void* stream);
+
+/* Group-limited routing: the experts form `groups` equal groups of
+ * neighbours; only the `top_groups` best groups (group_score, of the biased
+ * scores) are open, and the top-k are the best biased scores among their
+ * experts, best first, equal values by the lower index. Gates are
+ * bf16(score / sum of the picked scores) of the scores without the bias, 0
+ * where that sum is 0 (a softmax row without a finite logit has scores 0).
+ * E <= 256, groups <= 32 dividing E, k <= min(8, top_groups * E / groups).
+ * No counterpart in the reference, whose routers have no groups. */
+int praxis_b200_route_groups(const float* logits, const float* bias, int64_t tokens, int32_t experts, int32_t top_k,
+                             int32_t activation, int32_t groups, int32_t top_groups, int32_t group_score,
+                             int64_t* top_idx, void* gate, int device, void* stream);
 
 /* row_amax[r] = bf16(max |x[r, :]|) for bf16 x [rows, cols].
  * Replaces praxis/kernels/nvfp4_moe.py:15-21. */
@@ -397,6 +413,71 @@ typedef struct praxis_b200_expert_args {
 
 size_t praxis_b200_expert_workspace_size(int64_t rows, int32_t segments, int32_t dim, int32_t hidden);
 int praxis_b200_expert_forward(const praxis_b200_expert_args* args);
+
+/* ---- Block-scaled FP8 (E4M3) weights --------------------------------------
+ * No counterpart in the reference (its packed bank is NVFP4). For weights held
+ * in 8 bits with one fp32 scale per 128 x 128 block: w = q * scale. Activations
+ * are quantized in the call, one fp32 scale per 128 columns of a row:
+ *   a = max(max |x| of the block, 1e-12);  q = e4m3(x * f32(448 / a)) (round to
+ *   nearest even);  scale = f32(a / 448)
+ * Products are summed in fp32 per block of 128 columns and over the blocks.
+ * A NaN or an infinity in a row of x makes that row of the output NaN. */
+
+/* x [rows, cols] bf16 (row pitch ldx elements) -> q [rows, cols] E4M3 and
+ * scale[b * scale_ld + row] for block b of 128 columns (scale_ld >= rows).
+ * cols and ldx multiples of 16 and 8, x and q 16-byte aligned. */
+int praxis_b200_fp8_quantize(const void* x, int64_t rows, int32_t cols, int64_t ldx, void* q, float* scale,
+                             int64_t scale_ld, int device, void* stream);
+
+/* w [E, K, N] bf16 (input features first) -> q [E, N, K] E4M3 and scale
+ * [E, ceil(N / 128), ceil(K / 128)], the recipe above per 128 x 128 block.
+ * K % 16 == 0. */
+int praxis_b200_fp8_pack_weights(const void* w, int32_t experts, int32_t k, int32_t n, void* q, float* scale,
+                                 int device, void* stream);
+
+/* out [rows, n] bf16 = x [rows, k] (bf16, row pitch ldx) times the transposed
+ * weight w_q [n, k], w_scale [ceil(n / 128), ceil(k / 128)]. k % 16 == 0,
+ * ldx % 8 == 0, any n; x and w_q 16-byte aligned. */
+size_t praxis_b200_fp8_linear_workspace_size(int64_t rows, int32_t n, int32_t k);
+int praxis_b200_fp8_linear(const void* x, int64_t rows, int32_t k, int64_t ldx, const void* w_q, const float* w_scale,
+                           int32_t n, void* out, void* workspace, size_t workspace_size, int device, void* stream);
+
+/* A SwiGLU feed-forward on block-scaled weights, dense (a shared expert) or
+ * routed (top_k > 0): h = silu(x G^T) * (x U^T) in fp32, quantized per
+ * 128 columns as above, y = h D^T rounded to bf16. gate_up_q [E, 2F, C] holds
+ * G then U, gate_up_scale [E, 2F/128, C/128], down_q [E, C, F], down_scale
+ * [E, C/128, F/128]; dense: E = 1. Routed: the dispatch and the combine of
+ * praxis_b200_moe_forward (out[t] = bf16(sum of gate * scaling * y), then
+ * bf16(out + shared)). Dense: out = y; gate, scaling and shared are not used.
+ * C and F multiples of 128, buffers 16-byte aligned. */
+typedef struct praxis_b200_fp8_ffn_args {
+  const void* x;              /* [T, C] bf16 */
+  const int64_t* top_idx;     /* [T, k] */
+  const void* gate;           /* [T, k] bf16 */
+  const void* shared;         /* [T, C] bf16 or NULL */
+  void* out;                  /* [T, C] bf16 */
+  const void* gate_up_q;
+  const float* gate_up_scale;
+  const void* down_q;
+  const float* down_scale;
+  int64_t tokens;
+  int32_t dim;                /* C */
+  int32_t hidden;             /* F */
+  int32_t experts;            /* E */
+  int32_t top_k;              /* 0: dense */
+  float scaling;
+  void* workspace;
+  size_t workspace_size;
+  int device;
+  void* stream;
+  /* Optional, routed only: the combine fused into what follows the layer
+   * (praxis_b200_combine_tail); its outputs replace `out`, which may be NULL. */
+  const praxis_b200_tail* tail;
+} praxis_b200_fp8_ffn_args;
+
+/* top_k = 0: dense. */
+size_t praxis_b200_fp8_ffn_workspace_size(int64_t tokens, int32_t top_k, int32_t experts, int32_t dim, int32_t hidden);
+int praxis_b200_fp8_ffn(const praxis_b200_fp8_ffn_args* args);
 
 /* Dispatch without a caller workspace: praxis_b200_dispatch with the same
  * arguments (minus workspace / workspace_size) and the same outputs, its

@@ -8,6 +8,7 @@ Layers:
     capi    ctypes binding of include/praxis_b200_moe.h (the C ABI)
     ops     torch-facing functions, one per reference kernel function
     bank    B200NVFP4RoutedExperts, the drop-in routed bank
+    fp8     B200FP8RoutedExperts and FP8SharedExpert, experts in block-scaled FP8
     moe     B200MoEFeedForward, the MoE module
     expert_parallel  the bank sharded over GPUs with an all-to-all exchange
     pipeline  host-resident batches with copies overlapped with compute
@@ -20,11 +21,12 @@ from __future__ import annotations
 
 import sys
 
-from . import build, capi, expert_parallel, graphs, ops, pipeline, torch_ops  # noqa: F401
+from . import build, capi, expert_parallel, fp8, graphs, ops, pipeline, torch_ops  # noqa: F401
 from .bank import B200NVFP4RoutedExperts, pack_routed_experts, routed_forward_tail  # noqa: F401
+from .fp8 import B200FP8RoutedExperts, FP8SharedExpert, pack_routed_experts_fp8  # noqa: F401
 from .moe import B200MoEFeedForward  # noqa: F401
 
 sys.modules.setdefault("praxis_b200", sys.modules[__name__])
 
 __all__ = ["B200NVFP4RoutedExperts", "B200MoEFeedForward", "pack_routed_experts", "routed_forward_tail",
-           "build", "capi", "ops", "expert_parallel", "graphs", "pipeline", "torch_ops"]
+           "B200FP8RoutedExperts", "FP8SharedExpert", "pack_routed_experts_fp8", "build", "capi", "fp8", "ops", "expert_parallel", "graphs", "pipeline", "torch_ops"]

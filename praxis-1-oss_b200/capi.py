@@ -28,6 +28,7 @@ OK, EINVAL, ECUDA, EUNSUPPORTED = 0, 1, 2, 3
 SIGMOID, SOFTMAX = 0, 1
 EPI_PLAIN, EPI_SWIGLU, EPI_RESCALE = 0, 1, 2
 SF_COMPACT, SF_REPLICATED = 0, 1
+GROUP_TOP2, GROUP_MAX = 0, 1
 
 
 class MoeArgs(C.Structure):
@@ -119,6 +120,33 @@ class ExpertArgs(C.Structure):
     ]
 
 
+class Fp8FfnArgs(C.Structure):
+    """``praxis_b200_fp8_ffn_args``."""
+
+    _fields_ = [
+        ("x", P),
+        ("top_idx", P),
+        ("gate", P),
+        ("shared", P),
+        ("out", P),
+        ("gate_up_q", P),
+        ("gate_up_scale", P),
+        ("down_q", P),
+        ("down_scale", P),
+        ("tokens", I64),
+        ("dim", I32),
+        ("hidden", I32),
+        ("experts", I32),
+        ("top_k", I32),
+        ("scaling", F32),
+        ("workspace", P),
+        ("workspace_size", SZ),
+        ("device", C.c_int),
+        ("stream", P),
+        ("tail", P),
+    ]
+
+
 # name -> (restype, argtypes); the order and types follow the header.
 SIGNATURES: dict[str, tuple] = {
     "praxis_b200_abi_version": (C.c_int, []),
@@ -128,6 +156,10 @@ SIGNATURES: dict[str, tuple] = {
     "praxis_b200_padded_rows": (I64, [I64, I32]),
     "praxis_b200_router_logits": (C.c_int, [P, P, I32, I64, I32, I32, P, P, C.c_int, P]),
     "praxis_b200_route": (C.c_int, [P, P, I64, I32, I32, I32, P, P, C.c_int, P]),
+    "praxis_b200_route_groups": (
+        C.c_int,
+        [P, P, I64, I32, I32, I32, I32, I32, I32, P, P, C.c_int, P],
+    ),
     "praxis_b200_row_amax": (C.c_int, [P, I64, I32, P, C.c_int, P]),
     "praxis_b200_dispatch_workspace_size": (SZ, [I64, I32, I32]),
     "praxis_b200_dispatch_passes_workspace_size": (SZ, [I64, I32, I32, I32]),
@@ -168,6 +200,12 @@ SIGNATURES: dict[str, tuple] = {
     "praxis_b200_moe_forward": (C.c_int, [C.POINTER(MoeArgs)]),
     "praxis_b200_expert_workspace_size": (SZ, [I64, I32, I32, I32]),
     "praxis_b200_expert_forward": (C.c_int, [C.POINTER(ExpertArgs)]),
+    "praxis_b200_fp8_quantize": (C.c_int, [P, I64, I32, I64, P, P, I64, C.c_int, P]),
+    "praxis_b200_fp8_pack_weights": (C.c_int, [P, I32, I32, I32, P, P, C.c_int, P]),
+    "praxis_b200_fp8_linear_workspace_size": (SZ, [I64, I32, I32]),
+    "praxis_b200_fp8_linear": (C.c_int, [P, I64, I32, I64, P, P, I32, P, P, SZ, C.c_int, P]),
+    "praxis_b200_fp8_ffn_workspace_size": (SZ, [I64, I32, I32, I32, I32]),
+    "praxis_b200_fp8_ffn": (C.c_int, [C.POINTER(Fp8FfnArgs)]),
     "praxis_b200_dispatch_noalloc": (
         C.c_int,
         [P, P, P, I64, I32, I32, P, P, P, P, P, P, P, P, P, I32, P, P, P, C.c_int, P],

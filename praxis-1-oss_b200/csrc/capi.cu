@@ -37,6 +37,9 @@ int run_router_logits(const uint16_t* x, const uint16_t* w, int splits, int64_t 
                       float* logits, uint16_t* row_amax, cudaStream_t stream);
 int run_route(const float* logits, const float* bias, int64_t tokens, int experts, int top_k, int activation,
               int64_t* top_idx, uint16_t* gate, cudaStream_t stream);
+int run_route_groups(const float* logits, const float* bias, int64_t tokens, int experts, int top_k, int activation,
+                     int groups, int top_groups, int group_score, int64_t* top_idx, uint16_t* gate,
+                     cudaStream_t stream);
 int run_rescale_swiglu(const uint16_t* raw, int64_t rows, int hidden, const int32_t* pcsr, int experts,
                        const float* act_global, const float* w_global, uint16_t* out, uint16_t* rowmax, int alu,
                        cudaStream_t stream);
@@ -209,6 +212,57 @@ static ExpertLayout expert_layout(int64_t rows, int segments, int dim, int hidde
   return L;
 }
 
+// Workspace of the FP8 products. Dense linear: the quantized rows alone.
+struct Fp8LinearLayout {
+  size_t q, scale, total;
+  int64_t scale_ld;
+};
+
+static Fp8LinearLayout fp8_linear_layout(int64_t rows, int64_t k) {
+  Fp8LinearLayout L;
+  L.scale_ld = (rows + 31) / 32 * 32;
+  L.q = 0;
+  L.scale = ((size_t)rows * k + 255) & ~(size_t)255;
+  L.total = L.scale + (size_t)((k + 127) / 128) * L.scale_ld * 4;
+  return L;
+}
+
+// The feed-forward: `rows` are the tokens (dense) or the padded routed rows.
+struct Fp8FfnLayout {
+  size_t dispatch, inverse, csr, pcsr, offsets, tiles, num_tiles, aq, as, hq, hs, rows, total;
+  int64_t rp, scale_ld;
+  int max_tiles;
+};
+
+static Fp8FfnLayout fp8_ffn_layout(int64_t tokens, int top_k, int experts, int dim, int hidden) {
+  Fp8FfnLayout L;
+  size_t off = 0;
+  auto take = [&](size_t bytes) {
+    const size_t o = off;
+    off = (off + bytes + 255) & ~(size_t)255;
+    return o;
+  };
+  const bool routed = top_k > 0;
+  const int64_t r = tokens * top_k;
+  L.rp = routed ? padded_rows(r, experts) : tokens;
+  L.scale_ld = (L.rp + 31) / 32 * 32;
+  L.max_tiles = routed ? (int)(L.rp / 128) : 0;
+  L.dispatch = take(routed ? dispatch_workspace_bytes(tokens, top_k, experts) : 0);
+  L.inverse = take((size_t)r * 8);
+  L.csr = take(routed ? (size_t)(experts + 1) * 4 : 0);
+  L.pcsr = take(routed ? (size_t)(experts + 1) * 4 : 0);
+  L.offsets = take(routed ? (size_t)experts * 4 : 0);
+  L.tiles = take(routed ? (size_t)(2 * L.max_tiles + 1) * sizeof(TileEntry) : 0);
+  L.num_tiles = take(8);
+  L.aq = take((size_t)L.rp * dim);
+  L.as = take((size_t)(dim / 128) * L.scale_ld * 4);
+  L.hq = take((size_t)L.rp * hidden);
+  L.hs = take((size_t)(hidden / 128) * L.scale_ld * 4);
+  L.rows = take(routed ? (size_t)L.rp * dim * 2 : 0);
+  L.total = off;
+  return L;
+}
+
 }  // namespace praxis
 
 using namespace praxis;
@@ -257,6 +311,15 @@ int praxis_b200_route(const float* logits, const float* bias, int64_t tokens, in
   if (tokens > 0 && (!logits || !top_idx || !gate)) return set_error(PRAXIS_B200_EINVAL, "route: null pointer");
   return run_route(logits, bias, tokens, experts, top_k, activation, top_idx, static_cast<uint16_t*>(gate),
                    PRAXIS_STREAM(stream));
+}
+
+int praxis_b200_route_groups(const float* logits, const float* bias, int64_t tokens, int32_t experts, int32_t top_k,
+                             int32_t activation, int32_t groups, int32_t top_groups, int32_t group_score,
+                             int64_t* top_idx, void* gate, int device, void* stream) {
+  PRAXIS_DEVICE_OR_RETURN(device);
+  if (tokens > 0 && (!logits || !top_idx || !gate)) return set_error(PRAXIS_B200_EINVAL, "route_groups: null pointer");
+  return run_route_groups(logits, bias, tokens, experts, top_k, activation, groups, top_groups, group_score, top_idx,
+                          static_cast<uint16_t*>(gate), PRAXIS_STREAM(stream));
 }
 
 int praxis_b200_row_amax(const void* x, int64_t rows, int32_t cols, void* out, int device, void* stream) {
@@ -632,6 +695,169 @@ int praxis_b200_moe_forward(const praxis_b200_moe_args* a) {
   return run_combine(rows, a->dim, inverse, a->top_idx, gate, csr, pcsr, nullptr, h_amax, a->down_global, 1,
                      a->scaling, static_cast<const uint16_t*>(a->shared), static_cast<uint16_t*>(a->out), a->tokens,
                      a->top_k, a->experts, s, passes);
+}
+
+// ---------------------------------------------------------------------------
+// Block-scaled FP8 products
+// ---------------------------------------------------------------------------
+// Rows and columns that the kernels index: 32-bit tile coordinates.
+static int fp8_check(const char* what, int64_t rows, int64_t n, int64_t k) {
+  if (rows < 0 || rows > 0x7fffff00ll || n < 1 || k < 16 || k % 16 != 0)
+    return set_error(PRAXIS_B200_EINVAL, "%s: needs 0..2^31 rows, n >= 1 and a k that is a multiple of 16 (%lld, %lld, %lld)",
+                     what, (long long)rows, (long long)n, (long long)k);
+  if (((rows + 127) / 128) * ((n + 255) / 256) > 0x7fffffffll)
+    return set_error(PRAXIS_B200_EINVAL, "%s: too many output tiles", what);
+  return PRAXIS_B200_OK;
+}
+
+int praxis_b200_fp8_quantize(const void* x, int64_t rows, int32_t cols, int64_t ldx, void* q, float* scale,
+                             int64_t scale_ld, int device, void* stream) {
+  PRAXIS_DEVICE_OR_RETURN(device);
+  const int rc = fp8_check("fp8_quantize", rows, 1, cols);
+  if (rc) return rc;
+  if (rows == 0) return PRAXIS_B200_OK;
+  if (!x || !q || !scale) return set_error(PRAXIS_B200_EINVAL, "fp8_quantize: null pointer");
+  if (ldx < cols || ldx % 8 != 0 || scale_ld < rows || (((uintptr_t)x | (uintptr_t)q) & 15))
+    return set_error(PRAXIS_B200_EINVAL, "fp8_quantize: row pitch or alignment");
+  return run_fp8_quantize(static_cast<const uint16_t*>(x), rows, cols, ldx, Fp8Rows{}, static_cast<uint8_t*>(q), scale,
+                          scale_ld, PRAXIS_STREAM(stream));
+}
+
+int praxis_b200_fp8_pack_weights(const void* w, int32_t experts, int32_t k, int32_t n, void* q, float* scale,
+                                 int device, void* stream) {
+  PRAXIS_DEVICE_OR_RETURN(device);
+  if (!w || !q || !scale) return set_error(PRAXIS_B200_EINVAL, "fp8_pack_weights: null pointer");
+  if (experts < 1 || n < 1 || k < 16 || k % 16 != 0 ||
+      (int64_t)experts * ((n + 127) / 128) * ((k + 127) / 128) > 0x7fffffffll || ((uintptr_t)q & 3))
+    return set_error(PRAXIS_B200_EINVAL, "fp8_pack_weights: bad sizes (K must be a multiple of 16)");
+  return run_fp8_pack(static_cast<const uint16_t*>(w), experts, k, n, static_cast<uint8_t*>(q), scale,
+                      PRAXIS_STREAM(stream));
+}
+
+size_t praxis_b200_fp8_linear_workspace_size(int64_t rows, int32_t n, int32_t k) {
+  (void)n;
+  return rows < 0 || k < 0 ? 0 : fp8_linear_layout(rows, k).total;
+}
+
+int praxis_b200_fp8_linear(const void* x, int64_t rows, int32_t k, int64_t ldx, const void* w_q, const float* w_scale,
+                           int32_t n, void* out, void* workspace, size_t workspace_size, int device, void* stream) {
+  PRAXIS_DEVICE_OR_RETURN(device);
+  int rc = fp8_check("fp8_linear", rows, n, k);
+  if (rc) return rc;
+  if (rows == 0) return PRAXIS_B200_OK;
+  if (!x || !w_q || !w_scale || !out || !workspace) return set_error(PRAXIS_B200_EINVAL, "fp8_linear: null pointer");
+  if (ldx < k || ldx % 8 != 0 || (((uintptr_t)x | (uintptr_t)w_q | (uintptr_t)workspace) & 15) || ((uintptr_t)out & 1))
+    return set_error(PRAXIS_B200_EINVAL, "fp8_linear: row pitch or alignment");
+  const Fp8LinearLayout L = fp8_linear_layout(rows, k);
+  if (workspace_size < L.total)
+    return set_error(PRAXIS_B200_EINVAL, "fp8_linear: workspace %zu < %zu bytes", workspace_size, L.total);
+  cudaStream_t s = PRAXIS_STREAM(stream);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  float* scale = reinterpret_cast<float*>(ws + L.scale);
+  rc = run_fp8_quantize(static_cast<const uint16_t*>(x), rows, k, ldx, Fp8Rows{}, ws + L.q, scale, L.scale_ld, s);
+  if (rc) return rc;
+  Fp8Gemm g = {};
+  g.q = ws + L.q;
+  g.xs = scale;
+  g.xs_ld = L.scale_ld;
+  g.wq = static_cast<const uint8_t*>(w_q);
+  g.ws = w_scale;
+  g.rows = rows;
+  g.n = n;
+  g.k = k;
+  g.experts = 1;
+  g.out = static_cast<uint16_t*>(out);
+  return run_fp8_gemm(g, s);
+}
+
+size_t praxis_b200_fp8_ffn_workspace_size(int64_t tokens, int32_t top_k, int32_t experts, int32_t dim, int32_t hidden) {
+  if (tokens < 0 || top_k < 0 || experts < 1 || dim < 0 || hidden < 0) return 0;
+  return fp8_ffn_layout(tokens, top_k, experts, dim, hidden).total;
+}
+
+int praxis_b200_fp8_ffn(const praxis_b200_fp8_ffn_args* a) {
+  if (!a) return set_error(PRAXIS_B200_EINVAL, "fp8_ffn: null args");
+  PRAXIS_DEVICE_OR_RETURN(a->device);
+  const bool routed = a->top_k != 0;
+  if (a->dim < 128 || a->hidden < 128 || a->dim % 128 || a->hidden % 128)
+    return set_error(PRAXIS_B200_EINVAL, "fp8_ffn: C and F must be multiples of 128");
+  if (a->experts < 1 || (routed ? a->top_k < 0 || a->top_k > 8 || a->top_k > a->experts : a->experts != 1))
+    return set_error(PRAXIS_B200_EINVAL, "fp8_ffn: needs top_k 1..min(8, E), or one expert and no routing");
+  if (a->tokens < 0 || a->tokens * (int64_t)(routed ? a->top_k : 1) >= 0x7f000000ll)
+    return set_error(PRAXIS_B200_EINVAL, "fp8_ffn: too many rows");
+  const int top_k = a->top_k;
+  const Fp8FfnLayout L = fp8_ffn_layout(a->tokens, top_k, a->experts, a->dim, a->hidden);
+  int rc = fp8_check("fp8_ffn", L.rp, 2 * (int64_t)a->hidden > a->dim ? 2 * (int64_t)a->hidden : a->dim, a->dim);
+  if (rc) return rc;
+  if ((int64_t)a->experts * 2 * a->hidden > 0x7fffffffll || (int64_t)a->experts * a->dim > 0x7fffffffll)
+    return set_error(PRAXIS_B200_EINVAL, "fp8_ffn: too many weight rows");
+  if (a->tokens == 0) return PRAXIS_B200_OK;
+  if (a->tail && !routed) return set_error(PRAXIS_B200_EINVAL, "fp8_ffn: the tail follows routed experts");
+  if (!a->x || (!a->out && !a->tail) || !a->gate_up_q || !a->gate_up_scale || !a->down_q || !a->down_scale ||
+      !a->workspace || (routed && (!a->top_idx || !a->gate)))
+    return set_error(PRAXIS_B200_EINVAL, "fp8_ffn: null pointer");
+  if (((uintptr_t)a->x | (uintptr_t)a->out | (uintptr_t)a->gate_up_q | (uintptr_t)a->down_q | (uintptr_t)a->shared |
+       (uintptr_t)a->workspace) & 15)
+    return set_error(PRAXIS_B200_EINVAL, "fp8_ffn: buffers must be 16-byte aligned");
+  if (a->workspace_size < L.total)
+    return set_error(PRAXIS_B200_EINVAL, "fp8_ffn: workspace %zu < %zu bytes", a->workspace_size, L.total);
+  cudaStream_t s = PRAXIS_STREAM(a->stream);
+  uint8_t* ws = static_cast<uint8_t*>(a->workspace);
+  int64_t* inverse = reinterpret_cast<int64_t*>(ws + L.inverse);
+  int32_t* csr = reinterpret_cast<int32_t*>(ws + L.csr);
+  int32_t* pcsr = reinterpret_cast<int32_t*>(ws + L.pcsr);
+  TileEntry* tiles = reinterpret_cast<TileEntry*>(ws + L.tiles);
+  int32_t* num_tiles = reinterpret_cast<int32_t*>(ws + L.num_tiles);
+  float* as = reinterpret_cast<float*>(ws + L.as);
+  float* hs = reinterpret_cast<float*>(ws + L.hs);
+  uint16_t* rows = routed ? reinterpret_cast<uint16_t*>(ws + L.rows) : static_cast<uint16_t*>(a->out);
+  Fp8Rows to = {};
+  if (routed) {
+    rc = run_dispatch(a->top_idx, static_cast<const uint16_t*>(a->gate), nullptr, a->tokens, top_k, a->experts,
+                      Passes{1, 0}, ws + L.dispatch, L.inverse - L.dispatch, nullptr, inverse, nullptr, nullptr,
+                      nullptr, reinterpret_cast<int32_t*>(ws + L.offsets), csr, pcsr, tiles, L.max_tiles, num_tiles,
+                      nullptr, nullptr, s);
+    if (rc) return rc;
+    to = Fp8Rows{a->top_idx, inverse, csr, pcsr, top_k, a->experts};
+  }
+  rc = run_fp8_quantize(static_cast<const uint16_t*>(a->x), a->tokens, a->dim, a->dim, to, ws + L.aq, as, L.scale_ld,
+                        s);
+  if (rc) return rc;
+  Fp8Gemm g = {};
+  g.q = ws + L.aq;
+  g.xs = as;
+  g.xs_ld = L.scale_ld;
+  g.wq = static_cast<const uint8_t*>(a->gate_up_q);
+  g.ws = a->gate_up_scale;
+  g.rows = L.rp;
+  g.n = 2 * a->hidden;
+  g.k = a->dim;
+  g.experts = a->experts;
+  g.tiles = routed ? tiles : nullptr;
+  g.num_tiles = num_tiles;
+  g.max_tiles = L.max_tiles;
+  g.mean_rows = routed ? a->tokens * top_k / a->experts : 0;
+  g.hq = ws + L.hq;
+  g.hs = hs;
+  g.hs_ld = L.scale_ld;
+  rc = run_fp8_gemm(g, s);
+  if (rc) return rc;
+  g.q = ws + L.hq;
+  g.xs = hs;
+  g.wq = static_cast<const uint8_t*>(a->down_q);
+  g.ws = a->down_scale;
+  g.n = a->dim;
+  g.k = a->hidden;
+  g.out = rows;
+  rc = run_fp8_gemm(g, s);
+  if (rc || !routed) return rc;
+  if (a->tail != nullptr)
+    return run_combine_tail(rows, a->dim, inverse, a->top_idx, static_cast<const uint16_t*>(a->gate), csr, pcsr,
+                            nullptr, nullptr, nullptr, 1, a->scaling, static_cast<const uint16_t*>(a->shared),
+                            tail_args(*a->tail), a->tokens, top_k, a->experts, s);
+  return run_combine(rows, a->dim, inverse, a->top_idx, static_cast<const uint16_t*>(a->gate), csr, pcsr, nullptr,
+                     nullptr, nullptr, 1, a->scaling, static_cast<const uint16_t*>(a->shared),
+                     static_cast<uint16_t*>(a->out), a->tokens, top_k, a->experts, s);
 }
 
 // ---------------------------------------------------------------------------

@@ -10,4 +10,5 @@
 #include "combine.cu"
 #include "tail.cu"
 #include "swiglu.cu"
+#include "fp8.cu"
 #include "capi.cu"

@@ -407,6 +407,138 @@ __global__ void __launch_bounds__(256) route_kernel(const float* __restrict__ lo
 }
 
 // ---------------------------------------------------------------------------
+// Group-limited routing (experts <= 256 in at most 32 equal groups, top_k <= 8)
+//
+//   s = sigmoid(l) or softmax(l);  c = s + bias
+//   a group's score: the sum of its two best c, or its best c
+//   top = the k best c among the experts of the `top_groups` best groups,
+//         best first; equal values: the lower group or expert index
+//   gate = bf16(s[top] / sum), 0 where the sum is 0
+//
+// One warp per token. LPG = 32 / 2^ceil(log2 groups) neighbouring lanes share
+// a group and each holds up to P of its experts in a row, so a group's two
+// best are log2(LPG) shuffle merges and a closed group is whole lanes. Every
+// pick is a lane-local maximum and two warp reductions (redux.sync): the
+// largest value, as an order-preserving integer, then the lowest index with
+// that value. The scores are those of route_kernel's sigmoid; the softmax sum
+// is held in 64 bits and rounded once, so that its order moves no comparison.
+// ---------------------------------------------------------------------------
+template <int P>
+__global__ void __launch_bounds__(256) route_groups_kernel(const float* __restrict__ logits,
+                                                           const float* __restrict__ bias, int64_t tokens, int experts,
+                                                           int top_k, int activation, int groups, int top_groups,
+                                                           int top2, int lpg_log2, int64_t* __restrict__ top_idx,
+                                                           uint16_t* __restrict__ gate) {
+  pdl_wait();  // the previous kernel of the stream has completed
+  pdl_trigger();
+  constexpr uint32_t kAll = 0xffffffffu;
+  const int lane = threadIdx.x & 31;
+  const int64_t t = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  if (t >= tokens) return;
+  const int size = experts / groups, lpg = 1 << lpg_log2;
+  const int group = lane >> lpg_log2, part = lane & (lpg - 1);
+  const int per = (size + lpg - 1) >> lpg_log2;  // experts per lane, <= P
+  const int in_group = part * per;
+  const int mine = group < groups ? max(0, min(per, size - in_group)) : 0;
+  const int e0 = group * size + in_group;
+  const float* lr = logits + t * experts + e0;
+  float score[P];
+  float lmax = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    score[i] = i < mine ? lr[i] : -INFINITY;
+    lmax = fmaxf(lmax, score[i]);
+  }
+  if (activation == PRAXIS_B200_SOFTMAX) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) lmax = fmaxf(lmax, __shfl_xor_sync(kAll, lmax, o));
+    // a row without a finite logit has no scores: all 0
+    const bool none = lmax == -INFINITY;
+    double sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      score[i] = i < mine && !none ? expf(__fsub_rn(score[i], lmax)) : 0.0f;
+      sum += (double)score[i];
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kAll, sum, o);
+    const float total = none ? 1.0f : (float)sum;
+#pragma unroll
+    for (int i = 0; i < P; ++i) score[i] = div_rn(score[i], total);
+  } else {
+#pragma unroll
+    for (int i = 0; i < P; ++i) score[i] = div_rn(1.0f, add_rn(1.0f, expf(-score[i])));
+  }
+  // order-preserving keys of the biased scores; 0 (below every number) marks
+  // no expert, a closed group or a pick already made
+  uint32_t key[P];
+  uint32_t best = 0, second = 0;
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    key[i] = i < mine ? max(ordered_u32(bias != nullptr ? add_rn(score[i], bias[e0 + i]) : score[i]), 1u) : 0u;
+    second = max(second, min(best, key[i]));
+    best = max(best, key[i]);
+  }
+  uint32_t gkey = 0;
+  {
+    uint32_t b = best, s = second;
+    for (int o = 1; o < lpg; o <<= 1) {
+      const uint32_t ob = __shfl_xor_sync(kAll, b, o), os = __shfl_xor_sync(kAll, s, o);
+      s = max(max(s, os), min(b, ob));
+      b = max(b, ob);
+    }
+    if (group < groups)
+      gkey = max(top2 && s != 0 ? ordered_u32(add_rn(from_ordered_u32(b), from_ordered_u32(s))) : b, 1u);
+  }
+  bool open = false;
+  for (int j = 0; j < top_groups; ++j) {
+    const uint32_t m = __reduce_max_sync(kAll, gkey);
+    const int g = (int)__reduce_min_sync(kAll, gkey == m ? (uint32_t)group : 64u);
+    if (group == g) {
+      open = true;
+      gkey = 0;
+    }
+  }
+  if (!open) best = 0;
+  int my_idx = 0;
+  float my_score = 0.0f, total = 0.0f;
+  for (int j = 0; j < top_k; ++j) {
+    const uint32_t m = __reduce_max_sync(kAll, best);
+    // the lowest expert with that value: my lowest index, then the lowest lane
+    // (a lane's experts follow those of the lanes before it)
+    int at = 0;
+    float sc = 0.0f;
+    const uint32_t holders = __ballot_sync(kAll, best == m);
+    const int owner = __ffs(holders) - 1;
+    if (lane == owner) {
+#pragma unroll
+      for (int i = P - 1; i >= 0; --i)
+        if (key[i] == m) {
+          at = i;
+          sc = score[i];
+        }
+      best = 0;
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        if (i == at) key[i] = 0;
+        best = max(best, key[i]);
+      }
+    }
+    const int e = __shfl_sync(kAll, e0 + at, owner);
+    sc = __shfl_sync(kAll, sc, owner);
+    total = add_rn(total, sc);
+    if (lane == j) {
+      my_idx = e;
+      my_score = sc;
+    }
+  }
+  if (lane < top_k) {
+    top_idx[t * top_k + lane] = my_idx;
+    gate[t * top_k + lane] = f32_to_bf16(total == 0.0f ? 0.0f : div_rn(my_score, total));
+  }
+}
+
+// ---------------------------------------------------------------------------
 // Host entries
 // ---------------------------------------------------------------------------
 static int make_bf16_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int box_rows) {
@@ -483,6 +615,40 @@ int run_route(const float* logits, const float* bias, int64_t tokens, int expert
   launch_pdl(kernels[pi][top_k - 1], dim3(blocks), dim3(256), 0, stream, logits, bias, tokens, experts, activation,
              top_idx, gate);
   return check_launch("route");
+}
+
+int run_route_groups(const float* logits, const float* bias, int64_t tokens, int experts, int top_k, int activation,
+                     int groups, int top_groups, int group_score, int64_t* top_idx, uint16_t* gate,
+                     cudaStream_t stream) {
+  if (experts < 1 || experts > 256) return set_error(PRAXIS_B200_EINVAL, "routing supports 1..256 experts");
+  if (groups < 1 || groups > 32 || experts % groups != 0)
+    return set_error(PRAXIS_B200_EINVAL, "groups must be 1..32 and divide the experts (%d in %d groups)", experts, groups);
+  if (top_groups < 1 || top_groups > groups)
+    return set_error(PRAXIS_B200_EINVAL, "top_groups must be 1..%d", groups);
+  if (top_k < 1 || top_k > 8 || top_k > top_groups * (experts / groups))
+    return set_error(PRAXIS_B200_EINVAL, "top_k must be 1..min(8, experts of the open groups)");
+  if (activation != PRAXIS_B200_SIGMOID && activation != PRAXIS_B200_SOFTMAX)
+    return set_error(PRAXIS_B200_EINVAL, "unknown router activation");
+  if (group_score != PRAXIS_B200_GROUP_TOP2 && group_score != PRAXIS_B200_GROUP_MAX)
+    return set_error(PRAXIS_B200_EINVAL, "unknown group score");
+  if (tokens < 0) return set_error(PRAXIS_B200_EINVAL, "bad token count");
+  if (tokens == 0) return PRAXIS_B200_OK;
+  if ((tokens + 7) / 8 > 0x7fffffffll) return set_error(PRAXIS_B200_EINVAL, "too many tokens");
+  int lpg_log2 = 5;
+  while ((32 >> lpg_log2) < groups) --lpg_log2;
+  const int per = (experts / groups + (1 << lpg_log2) - 1) >> lpg_log2;
+  const dim3 grid((unsigned)((tokens + 7) / 8));
+  const int top2 = group_score == PRAXIS_B200_GROUP_TOP2;
+#define PRAXIS_ROUTE_GROUPS(P)                                                                                     \
+  launch_pdl(route_groups_kernel<P>, grid, dim3(256), 0, stream, logits, bias, tokens, experts, top_k, activation, \
+             groups, top_groups, top2, lpg_log2, top_idx, gate)
+  // experts per lane: 2^ceil(log2 groups) lanes' shares, at most 16 (256
+  // experts in 9 or 17 groups leave almost half of the lanes without one)
+  if (per <= 4) PRAXIS_ROUTE_GROUPS(4);
+  else if (per <= 8) PRAXIS_ROUTE_GROUPS(8);
+  else PRAXIS_ROUTE_GROUPS(16);
+#undef PRAXIS_ROUTE_GROUPS
+  return check_launch("route_groups");
 }
 
 }  // namespace praxis

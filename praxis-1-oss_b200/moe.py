@@ -12,6 +12,7 @@ routed sum is rounded to bf16.
 from __future__ import annotations
 
 import os
+from functools import partial
 
 import torch
 import torch.nn.functional as F
@@ -19,6 +20,7 @@ from torch import Tensor, nn
 
 from . import ops
 from .bank import B200NVFP4RoutedExperts, pack_routed_experts, routed_forward_tail
+from .fp8 import B200FP8RoutedExperts, FP8SharedExpert, pack_routed_experts_fp8
 from .ops import Tail
 
 _NVTX = os.environ.get("PRAXIS_NVTX", "0") not in ("", "0")
@@ -56,8 +58,12 @@ class SharedExpert(nn.Module):
 
 
 class B200MoEFeedForward(nn.Module):
-    """Router (sigmoid or softmax) + top-k routed NVFP4 experts + optional
-    shared expert, inference only.
+    """Router (sigmoid or softmax) + top-k routed experts (NVFP4, or
+    block-scaled FP8) + optional shared expert, inference only.
+
+    ``router_groups`` > 1: group-limited routing (``ops.route``): the picks
+    come from the ``router_top_groups`` best groups of experts, judged by
+    ``router_group_score`` ("top2" or "max").
 
     ``routing_hook`` (praxis/layers.py:1595-1602): None at inference; a
     callable ``hook(layer, logits, top_idx)`` set by training or diagnostics
@@ -79,21 +85,35 @@ class B200MoEFeedForward(nn.Module):
         *,
         router_activation: str = "sigmoid",
         shared_expert: bool = True,
+        router_groups: int = 1,
+        router_top_groups: int | None = None,
+        router_group_score: str = "top2",
     ) -> None:
         super().__init__()
         if dispatch_chunk_size is not None and dispatch_chunk_size <= 0:
             raise ValueError("dispatch_chunk_size must be positive")
         if router_activation not in ("sigmoid", "softmax"):
             raise ValueError("router_activation must be 'sigmoid' or 'softmax'")
+        if router_groups != 1 or router_top_groups is not None:
+            if not 1 <= router_groups <= 32 or num_experts % router_groups:
+                raise ValueError("router_groups must be 1..32 and divide the experts")
+            if router_top_groups is None or not 1 <= router_top_groups <= router_groups:
+                raise ValueError("router_top_groups must be 1..router_groups")
+            if top_k > router_top_groups * (num_experts // router_groups):
+                raise ValueError("top_k exceeds the experts of the open groups")
+        if router_group_score not in ("top2", "max"):
+            raise ValueError("router_group_score must be 'top2' or 'max'")
         self.dim, self.hidden = dim, hidden
         self.dispatch_chunk_size = dispatch_chunk_size
         self.num_experts = num_experts
         self.top_k = top_k
         self.routed_scaling_factor = routed_scaling_factor
         self.router_activation = router_activation
+        self.router_groups, self.router_top_groups = router_groups, router_top_groups
+        self.router_group_score = router_group_score
         self.router = nn.Linear(dim, num_experts, bias=False)
-        self.routed: B200NVFP4RoutedExperts | None = None
-        self.shared = SharedExpert(dim, hidden) if shared_expert else None
+        self.routed: B200NVFP4RoutedExperts | B200FP8RoutedExperts | None = None
+        self.shared: SharedExpert | FP8SharedExpert | None = SharedExpert(dim, hidden) if shared_expert else None
         self.register_buffer("expert_bias", torch.zeros(num_experts))
         self._router_terms: Tensor | None = None
 
@@ -105,9 +125,22 @@ class B200MoEFeedForward(nn.Module):
         self._router_terms = None
         return self
 
-    def set_routed_weights(self, gate_up_weight: Tensor, down_weight: Tensor) -> None:
-        """Pack expert-first bf16 banks [E,C,2H] / [E,H,C] on the GPU."""
-        self.routed = pack_routed_experts(gate_up_weight, down_weight, keep_on_device=True)
+    def set_routed_weights(self, gate_up_weight: Tensor, down_weight: Tensor, format: str = "nvfp4") -> None:
+        """Pack expert-first bf16 banks [E,C,2H] / [E,H,C] on the GPU as NVFP4
+        or as block-scaled FP8 (``format="fp8"``)."""
+        if format not in ("nvfp4", "fp8"):
+            raise ValueError("format must be 'nvfp4' or 'fp8'")
+        if format == "fp8":
+            self.routed = pack_routed_experts_fp8(gate_up_weight, down_weight)
+        else:
+            self.routed = pack_routed_experts(gate_up_weight, down_weight, keep_on_device=True)
+
+    def quantize_shared(self) -> None:
+        """Hold the bf16 shared expert's weights as block-scaled FP8 from here
+        on (on its CUDA device; C and H multiples of 128)."""
+        if not isinstance(self.shared, SharedExpert):
+            raise ValueError("there is no bf16 shared expert to quantize")
+        self.shared = FP8SharedExpert.from_weights(self.shared.gate_up, self.shared.down)
 
     @classmethod
     def from_reference(cls, layer: nn.Module) -> B200MoEFeedForward:
@@ -153,7 +186,8 @@ class B200MoEFeedForward(nn.Module):
             logits, _ = ops.router_logits(x_flat, self.router_terms())
         with _Range("topk_dispatch"):
             bias = self.expert_bias.to(device=x_flat.device, dtype=torch.float32).contiguous()
-            top_idx, gate = ops.route(logits, bias, self.top_k, self.router_activation)
+            top_idx, gate = ops.route(logits, bias, self.top_k, self.router_activation, groups=self.router_groups,
+                                      top_groups=self.router_top_groups, group_score=self.router_group_score)
         if self.routing_hook is not None:
             self.routing_hook(self, logits, top_idx)
         return top_idx, gate
@@ -213,8 +247,10 @@ class B200MoEFeedForward(nn.Module):
                                  mod_geom=None if geom is None else tuple(int(v) for v in geom))
         chunk = self.dispatch_chunk_size or max(1, x_flat.shape[0])
         with _Range("routed"):
-            xo, h = routed_forward_tail(self.routed, x_flat, top_idx, gate, scaling=self.routed_scaling_factor,
-                                        chunk_size=chunk, tail=tail, shared=y_shared)
+            run = (self.routed.routed_forward_tail if isinstance(self.routed, B200FP8RoutedExperts)
+                   else partial(routed_forward_tail, self.routed))
+            xo, h = run(x_flat, top_idx, gate, scaling=self.routed_scaling_factor, chunk_size=chunk, tail=tail,
+                        shared=y_shared)
         return xo.reshape(shape), None if h is None else h.reshape(shape)
 
     @torch.no_grad()
@@ -228,7 +264,7 @@ class B200MoEFeedForward(nn.Module):
         expert GEMMs once, grouped per (expert, input) so that every output
         has the bits of ``forward``. Falls back to one forward per input where
         the pair does not apply (the reference's conditions: two inputs, each
-        one dispatch chunk, no routing hook)."""
+        one dispatch chunk, no routing hook; and a bank that has the pair)."""
         xs = list(xs)
         if self.routed is None:
             raise RuntimeError("routed experts are not set (set_routed_weights / from_reference)")
@@ -236,6 +272,7 @@ class B200MoEFeedForward(nn.Module):
         chunk = self.dispatch_chunk_size
         if (
             len(xs) != 2
+            or not hasattr(self.routed, "routed_forward_pair")
             or self.routing_hook is not None
             or any(not f.is_cuda or f.dtype != torch.bfloat16 or f.device != flats[0].device for f in flats)
             or any(not 0 < f.shape[0] <= (chunk or f.shape[0]) for f in flats)

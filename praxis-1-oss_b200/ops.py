@@ -19,6 +19,7 @@ from torch import Tensor
 from . import capi
 
 BF16 = torch.bfloat16
+F8 = torch.float8_e4m3fn
 
 
 def _p(t: Tensor | None):
@@ -42,6 +43,20 @@ def _need(t: Tensor, name: str, dtype, ndim: int | None = None, device=None) -> 
         raise ValueError(f"{name}: expected {ndim} dims, got {t.ndim}")
     if device is not None and t.device != device:
         raise ValueError(f"{name}: tensors must share a device")
+
+
+_ACTIVATIONS = {"sigmoid": capi.SIGMOID, "softmax": capi.SOFTMAX}
+_GROUP_SCORES = {"top2": capi.GROUP_TOP2, "max": capi.GROUP_MAX}
+
+
+def _run(t: Tensor, fn, *args) -> None:
+    """Calls a C entry point, which makes ``t``'s device current, and gives
+    the caller its current device back."""
+    device = torch.cuda.current_device()
+    status = fn(*args)
+    if t.device.index != device:
+        torch.cuda.set_device(device)
+    capi.check(status)
 
 
 def padded_rows(routed_rows: int, experts: int) -> int:
@@ -100,17 +115,44 @@ def router_logits(x: Tensor, weight_terms: Tensor) -> tuple[Tensor, Tensor]:
     return logits, amax
 
 
-def route(logits: Tensor, bias: Tensor | None, top_k: int, activation: str = "sigmoid") -> tuple[Tensor, Tensor]:
-    """Gating + top-k + renormalised bf16 gates (praxis/layers.py:1647-1653)."""
+def route(logits: Tensor, bias: Tensor | None, top_k: int, activation: str = "sigmoid", *, groups: int = 1,
+          top_groups: int | None = None, group_score: str = "top2") -> tuple[Tensor, Tensor]:
+    """Gating + top-k + renormalised bf16 gates (praxis/layers.py:1647-1653).
+
+    With ``groups`` > 1 the routing is group-limited
+    (``praxis_b200_route_groups``): the experts form that many equal groups of
+    neighbours, the ``top_groups`` best ones are open (a group's score is the
+    sum of its two best biased scores, or with ``group_score="max"`` its best
+    one) and the top-k are taken among their experts, best first, ties by the
+    lower index. ``bias`` takes part in the choice only."""
     _need(logits, "logits", torch.float32, 2)
     if bias is not None:
         _need(bias, "expert bias", torch.float32, 1, logits.device)
+        if bias.numel() < logits.shape[1]:
+            raise ValueError("expert bias: one value per expert")
     t, e = logits.shape
-    act = {"sigmoid": capi.SIGMOID, "softmax": capi.SOFTMAX}[activation]
+    if activation not in _ACTIVATIONS:
+        raise ValueError("activation must be 'sigmoid' or 'softmax'")
+    act = _ACTIVATIONS[activation]
+    if top_k < 1 or top_k > e:
+        raise ValueError(f"top_k must be 1..{e}")
+    if group_score not in _GROUP_SCORES:
+        raise ValueError("group_score must be 'top2' or 'max'")
+    if groups == 1 and top_groups not in (None, 1):
+        raise ValueError("top_groups needs groups")
+    if groups != 1 and (not 1 <= groups <= 32 or e % groups or top_groups is None or not 1 <= top_groups <= groups
+                        or top_k > top_groups * (e // groups)):
+        raise ValueError("group-limited routing needs 1..32 equal groups, 1 <= top_groups <= groups and top_k within "
+                         "the experts of the open groups")
     top_idx = torch.empty(t, top_k, dtype=torch.int64, device=logits.device)
     gate = torch.empty(t, top_k, dtype=BF16, device=logits.device)
-    capi.check(capi.load().praxis_b200_route(
-        _p(logits), _p(bias), t, e, top_k, act, _p(top_idx), _p(gate), _dev(logits), _stream(logits)))
+    lib = capi.load()
+    if groups == 1:
+        capi.check(lib.praxis_b200_route(
+            _p(logits), _p(bias), t, e, top_k, act, _p(top_idx), _p(gate), _dev(logits), _stream(logits)))
+        return top_idx, gate
+    _run(logits, lib.praxis_b200_route_groups, _p(logits), _p(bias), t, e, top_k, act, groups, top_groups,
+         _GROUP_SCORES[group_score], _p(top_idx), _p(gate), _dev(logits), _stream(logits))
     return top_idx, gate
 
 
@@ -668,3 +710,190 @@ def moe_forward(x: Tensor, top_idx: Tensor | None, gate: Tensor | None, gate_up_
     if router_terms is not None:
         res = res + (top_idx, gate)
     return res if len(res) > 1 else out
+
+
+# -- block-scaled FP8 weights ------------------------------------------------
+def _fp8_weight(q: Tensor, scale: Tensor, name: str, ndim: int, device) -> None:
+    """E4M3 values [.., N, K] with one fp32 scale per 128 x 128 block."""
+    _need(q, name + "_q", F8, ndim, device)
+    _need(scale, name + "_scale", torch.float32, ndim, device)
+    n, k = q.shape[-2:]
+    want = q.shape[:-2] + (-(-n // 128), -(-k // 128))
+    if scale.shape != want:
+        raise ValueError(f"{name}_scale: expected {tuple(want)}, got {tuple(scale.shape)}")
+
+
+def _fp8_rows(x: Tensor, width: int) -> Tensor:
+    """x [.., width] as bf16 rows whose columns are neighbours."""
+    if not isinstance(x, Tensor) or x.dtype != BF16 or x.device.type != "cuda" or x.ndim < 1:
+        raise ValueError("x: expected a CUDA bf16 tensor")
+    if x.shape[-1] != width:
+        raise ValueError(f"x: expected {width} columns, got {x.shape[-1]}")
+    if x.ndim != 2:
+        if not x.is_contiguous():
+            raise ValueError("x: expected a contiguous tensor or rows of one pitch")
+        x = x.view(-1, width)
+    if x.numel() and (x.stride(1) != 1 or (x.shape[0] > 1 and (x.stride(0) < width or x.stride(0) % 8))
+                      or x.data_ptr() % 16):
+        raise ValueError("x: rows must be contiguous, 16-byte aligned and a multiple of 8 elements apart")
+    return x
+
+
+def _pitch(x: Tensor) -> int:
+    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+
+
+def fp8_quantize(x: Tensor) -> tuple[Tensor, Tensor]:
+    """The activation quantization of the FP8 products: (q E4M3 [R, K],
+    scale fp32 [R, ceil(K / 128)]) of bf16 rows x [R, K], K % 16 == 0. A block
+    of 128 columns with largest magnitude a = max(|x|, 1e-12) is held as
+    e4m3(x * f32(448 / a)) with scale f32(a / 448)."""
+    if not isinstance(x, Tensor) or x.ndim != 2:
+        raise ValueError("x: expected 2 dims")
+    x = _fp8_rows(x, x.shape[1])
+    r, k = x.shape
+    ld = -(-max(r, 1) // 32) * 32
+    q = torch.empty(r, k, dtype=F8, device=x.device)
+    scale = torch.empty(-(-k // 128), ld, dtype=torch.float32, device=x.device)
+    _run(x, capi.load().praxis_b200_fp8_quantize, _p(x), r, k, _pitch(x), _p(q), _p(scale), ld, _dev(x), _stream(x))
+    return q, scale[:, :r].T
+
+
+def fp8_pack_weights(w: Tensor) -> tuple[Tensor, Tensor]:
+    """Expert-first bf16 bank [E, K, N] (or one matrix [K, N]), input features
+    first -> (q E4M3 [.., N, K], scale fp32 [.., ceil(N/128), ceil(K/128)])
+    on the GPU, the recipe of :func:`fp8_quantize` per 128 x 128 block."""
+    if not isinstance(w, Tensor) or w.ndim not in (2, 3):
+        raise ValueError("weights: expected [E, K, N] or [K, N]")
+    _need(w, "weights", BF16)
+    e = w.shape[0] if w.ndim == 3 else 1
+    k, n = w.shape[-2:]
+    q = torch.empty(w.shape[:-2] + (n, k), dtype=F8, device=w.device)
+    scale = torch.empty(w.shape[:-2] + (-(-n // 128), -(-k // 128)), dtype=torch.float32, device=w.device)
+    _run(w, capi.load().praxis_b200_fp8_pack_weights, _p(w), e, k, n, _p(q), _p(scale), _dev(w), _stream(w))
+    return q, scale
+
+
+def fp8_linear(x: Tensor, w_q: Tensor, w_scale: Tensor) -> Tensor:
+    """``x @ W.T`` in bf16 for a block-scaled FP8 weight: W [N, K] is ``w_q``
+    (E4M3) times ``w_scale`` [ceil(N/128), ceil(K/128)] per 128 x 128 block.
+    x [.., K] bf16 (2-D rows may be a column slice of a wider tensor) is
+    quantized in the call as by :func:`fp8_quantize`; the products are summed
+    in fp32. K % 16 == 0, any N, any number of rows. Inference only."""
+    _fp8_weight(w_q, w_scale, "w", 2, None)
+    n, k = w_q.shape
+    rows = _fp8_rows(x, k)
+    _same_device(x, w_q, w_scale)
+    _inference_only(x)
+    r = rows.shape[0]
+    out = torch.empty(x.shape[:-1] + (n,), dtype=BF16, device=x.device)
+    lib = capi.load()
+    size = int(lib.praxis_b200_fp8_linear_workspace_size(r, n, k))
+    ws = torch.empty(size, dtype=torch.uint8, device=x.device)
+    _run(x, lib.praxis_b200_fp8_linear, _p(rows), r, k, _pitch(rows), _p(w_q), _p(w_scale), n, _p(out), _p(ws), size,
+         _dev(x), _stream(x))
+    return out
+
+
+def _same_device(x: Tensor, *others) -> None:
+    if any(t is not None and t.device != x.device for t in others):
+        raise ValueError("tensors must share a device")
+
+
+def _inference_only(*tensors) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError("the FP8 products support inference only")
+
+
+def _fp8_ffn_shapes(gate_up_q: Tensor, gate_up_scale: Tensor, down_q: Tensor, down_scale: Tensor, ndim: int
+                    ) -> tuple[int, int, int]:
+    """(E, C, F) of a gate/up and a down weight that belong together."""
+    _fp8_weight(gate_up_q, gate_up_scale, "gate_up", ndim, None)
+    _fp8_weight(down_q, down_scale, "down", ndim, gate_up_q.device)
+    _same_device(gate_up_q, gate_up_scale, down_scale)
+    f2, c = gate_up_q.shape[-2:]
+    f = f2 // 2
+    if f2 % 2 or c % 128 or f % 128 or not c or not f or down_q.shape != gate_up_q.shape[:-2] + (c, f):
+        raise ValueError("expected gate_up_q [.., 2F, C] and down_q [.., C, F], C and F multiples of 128")
+    return (gate_up_q.shape[0] if ndim == 3 else 1), c, f
+
+
+def _fp8_ffn(rows: Tensor, top_idx: Tensor | None, gate: Tensor | None, shared: Tensor | None, out: Tensor | None,
+             weights: tuple, sizes: tuple, scaling: float, tail=None) -> None:
+    e, c, f = sizes
+    t = rows.shape[0]
+    k = 0 if top_idx is None else top_idx.shape[1]
+    lib = capi.load()
+    size = int(lib.praxis_b200_fp8_ffn_workspace_size(t, k, e, c, f))
+    ws = torch.empty(size, dtype=torch.uint8, device=rows.device)
+    gate_up_q, gate_up_scale, down_q, down_scale = weights
+    args = capi.Fp8FfnArgs(
+        x=rows.data_ptr(), top_idx=_p(top_idx), gate=_p(gate), shared=_p(shared), out=_p(out),
+        gate_up_q=gate_up_q.data_ptr(), gate_up_scale=gate_up_scale.data_ptr(), down_q=down_q.data_ptr(),
+        down_scale=down_scale.data_ptr(), tokens=t, dim=c, hidden=f, experts=e, top_k=k, scaling=float(scaling),
+        workspace=ws.data_ptr(), workspace_size=size, device=_dev(rows),
+        stream=torch.cuda.current_stream(rows.device).cuda_stream,
+        tail=None if tail is None else C.addressof(tail))
+    _run(rows, lib.praxis_b200_fp8_ffn, C.byref(args))
+
+
+def fp8_mlp(x: Tensor, gate_up_q: Tensor, gate_up_scale: Tensor, down_q: Tensor, down_scale: Tensor, *,
+            out: Tensor | None = None) -> Tensor:
+    """A dense SwiGLU feed-forward (a shared expert) on block-scaled FP8
+    weights: ``(silu(x G^T) * (x U^T)) D^T`` in bf16, gate_up_q [2F, C] = G
+    then U, down_q [C, F], scales per 128 x 128 block. Both products quantize
+    their activations (:func:`fp8_quantize`); the hidden values go from fp32
+    to E4M3 without a rounding in between. Inference only."""
+    sizes = _fp8_ffn_shapes(gate_up_q, gate_up_scale, down_q, down_scale, 2)
+    if not isinstance(x, Tensor) or not x.is_contiguous():
+        raise ValueError("x: expected a contiguous CUDA bf16 tensor")
+    rows = _fp8_rows(x, sizes[1])
+    _same_device(x, gate_up_q)
+    _inference_only(x)
+    if out is None:
+        out = torch.empty_like(x)
+    else:
+        _need(out, "out", BF16, x.ndim, x.device)
+        if out.shape != x.shape:
+            raise ValueError("out must have the shape of x")
+    _fp8_ffn(rows, None, None, None, out, (gate_up_q, gate_up_scale, down_q, down_scale), sizes, 1.0)
+    return out
+
+
+def fp8_moe_forward(x: Tensor, top_idx: Tensor, gate: Tensor, gate_up_q: Tensor, gate_up_scale: Tensor,
+                    down_q: Tensor, down_scale: Tensor, scaling: float, shared: Tensor | None = None, *,
+                    out: Tensor | None = None, tail: Tail | None = None, tail_out: tuple | None = None):
+    """:func:`moe_forward` for routed experts on block-scaled FP8 weights
+    (gate_up_q [E, 2F, C], gate rows then up rows, down_q [E, C, F], scales
+    per 128 x 128 block): dispatch, quantization of each token's row once,
+    both expert products with SwiGLU and the hidden quantization between them,
+    weighted combine (+ ``shared``). With ``tail`` the result is ``(new
+    residual, normed rows or None)`` as there. Inference only."""
+    sizes = _fp8_ffn_shapes(gate_up_q, gate_up_scale, down_q, down_scale, 3)
+    e, c, _ = sizes
+    _need(x, "x", BF16, 2, gate_up_q.device)
+    t = x.shape[0]
+    if x.shape[1] != c:
+        raise ValueError(f"x: expected {c} columns, got {x.shape[1]}")
+    _need(top_idx, "top_idx", torch.int64, 2, x.device)
+    _need(gate, "gate", BF16, 2, x.device)
+    if top_idx.shape[0] != t or gate.shape != top_idx.shape or not 1 <= top_idx.shape[1] <= min(8, e):
+        raise ValueError("top_idx / gate: expected [T, k], 1 <= k <= min(8, E)")
+    if shared is not None:
+        _need(shared, "shared", BF16, 2, x.device)
+        if shared.shape != x.shape:
+            raise ValueError("shared must have the shape of x")
+    _inference_only(x, gate, shared)
+    weights = (gate_up_q, gate_up_scale, down_q, down_scale)
+    if tail is not None:
+        st, residual_out, normed = _tail_struct(tail, t, c, x.device, tail_out)
+        _fp8_ffn(x, top_idx, gate, shared, None, weights, sizes, scaling, st)
+        return residual_out, normed
+    if out is None:
+        out = torch.empty_like(x)
+    else:
+        _need(out, "out", BF16, 2, x.device)
+        if out.shape != x.shape:
+            raise ValueError("out must have the shape of x")
+    _fp8_ffn(x, top_idx, gate, shared, out, weights, sizes, scaling)
+    return out

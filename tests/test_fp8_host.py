@@ -1,0 +1,198 @@
+"""What the block-scaled FP8 products and the group-limited router refuse,
+without a GPU (fake CUDA tensors; nothing is launched)."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+from conftest import pkg
+from torch._subclasses.fake_tensor import FakeTensorMode
+
+BF16 = torch.bfloat16
+F8 = torch.float8_e4m3fn
+
+
+def cuda(*shape, dtype=BF16):
+    return torch.empty(*shape, dtype=dtype, device="cuda")
+
+
+def weight(*shape):
+    n, k = shape[-2:]
+    return cuda(*shape, dtype=F8), cuda(*shape[:-2], -(-n // 128), -(-k // 128), dtype=torch.float32)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(groups=3, top_groups=1), dict(groups=4), dict(groups=4, top_groups=5), dict(groups=4, top_groups=0),
+    dict(groups=0, top_groups=1), dict(groups=64, top_groups=1), dict(top_groups=2),
+    dict(groups=16, top_groups=1), dict(groups=4, top_groups=2, group_score="mean"),
+])
+def test_route_refuses_bad_groups(kw):
+    with FakeTensorMode(), pytest.raises(ValueError):
+        pkg().ops.route(cuda(5, 64, dtype=torch.float32), None, 6, "sigmoid", **kw)
+
+
+def test_route_refuses_bad_arguments():
+    with FakeTensorMode():
+        logits = cuda(5, 64, dtype=torch.float32)
+        for args in ((logits, None, 4, "tanh"), (logits, None, 0, "sigmoid"), (logits, None, 65, "sigmoid"),
+                     (logits, cuda(63, dtype=torch.float32), 4, "sigmoid"), (logits.to(BF16), None, 4, "sigmoid")):
+            with pytest.raises(ValueError):
+                pkg().ops.route(*args, groups=4, top_groups=2)
+
+
+@pytest.mark.parametrize("kind", ["dtype", "width", "columns", "scale_shape", "scale_dtype", "weight_dtype",
+                                  "weight_strided", "cpu", "transposed", "pitch"])
+def test_linear_refuses(kind):
+    with FakeTensorMode():
+        x, (q, s) = cuda(4, 256), weight(300, 256)
+        if kind == "dtype":
+            x = x.float()
+        elif kind == "width":
+            x = cuda(4, 128)
+        elif kind == "columns":
+            x = cuda(4, 512)[:, ::2]
+        elif kind == "scale_shape":
+            s = s[:2].contiguous()
+        elif kind == "scale_dtype":
+            s = s.to(BF16)
+        elif kind == "weight_dtype":
+            q = q.to(BF16)
+        elif kind == "weight_strided":
+            q = cuda(256, 300, dtype=F8).T
+        elif kind == "cpu":
+            x = torch.empty(4, 256, dtype=BF16)
+        elif kind == "transposed":
+            x = cuda(256, 4).T
+        else:
+            x = cuda(4, 260)[:, :256]  # rows 260 elements apart are not 16-byte aligned
+        with pytest.raises(ValueError):
+            pkg().ops.fp8_linear(x, q, s)
+
+
+def test_products_refuse_gradients():
+    with FakeTensorMode():
+        q, s = weight(128, 256)
+        with pytest.raises(RuntimeError, match="inference"):
+            pkg().ops.fp8_linear(cuda(4, 256).requires_grad_(), q, s)
+
+
+@pytest.mark.parametrize("kind", ["odd", "small", "down", "out", "x_strided", "experts"])
+def test_mlp_refuses(kind):
+    with FakeTensorMode():
+        c, f = 256, 384
+        x, gu, down, out = cuda(4, c), weight(2 * f, c), weight(c, f), None
+        if kind == "odd":
+            gu = weight(2 * f + 1, c)
+        elif kind == "small":
+            gu, down = weight(2 * 64, c), weight(c, 64)
+        elif kind == "down":
+            down = weight(c, 256)
+        elif kind == "out":
+            out = cuda(3, c)
+        elif kind == "x_strided":
+            x = cuda(4, 2 * c)[:, :c]
+        else:
+            gu, down = weight(2, 2 * f, c), weight(2, c, f)
+        with pytest.raises(ValueError):
+            pkg().ops.fp8_mlp(x, *gu, *down, out=out)
+
+
+@pytest.mark.parametrize("kind", ["top_dtype", "top_k", "gate_shape", "gate_dtype", "shared", "tokens", "width", "out"])
+def test_moe_forward_refuses(kind):
+    with FakeTensorMode():
+        e, c, f, t, k = 4, 256, 128, 6, 2
+        x, top, gate, shared, out = cuda(t, c), cuda(t, k, dtype=torch.int64), cuda(t, k), None, None
+        if kind == "top_dtype":
+            top = top.to(torch.int32)
+        elif kind == "top_k":
+            top, gate = cuda(t, 5, dtype=torch.int64), cuda(t, 5)
+        elif kind == "gate_shape":
+            gate = cuda(t, 1)
+        elif kind == "gate_dtype":
+            gate = gate.float()
+        elif kind == "shared":
+            shared = cuda(t, 128)
+        elif kind == "tokens":
+            x = cuda(t + 1, c)
+        elif kind == "width":
+            x = cuda(t, 128)
+        else:
+            out = cuda(t, c, dtype=torch.float32)
+        with pytest.raises(ValueError):
+            pkg().ops.fp8_moe_forward(x, top, gate, *weight(e, 2 * f, c), *weight(e, c, f), 1.0, shared, out=out)
+
+
+def packed(e=2, c=128, f=128):
+    return {
+        "gate_up_q": torch.zeros(e, 2 * f, c).to(F8), "gate_up_scale": torch.ones(e, 2 * f // 128, c // 128),
+        "down_q": torch.zeros(e, c, f).to(F8), "down_scale": torch.ones(e, c // 128, f // 128),
+    }
+
+
+@pytest.mark.parametrize("kind", ["missing", "extra", "shape", "dtype", "scale_nan", "scale_zero", "value_nan", "odd"])
+def test_bank_rejects_corrupt_state(kind):
+    state = packed()
+    if kind == "missing":
+        del state["down_q"]
+    elif kind == "extra":
+        state["bias"] = torch.ones(1)
+    elif kind == "shape":
+        state["down_q"] = state["down_q"][:, :, :64].contiguous()
+    elif kind == "dtype":
+        state["down_scale"] = state["down_scale"].to(BF16)
+    elif kind.startswith("scale"):
+        state["gate_up_scale"][0, 0, 0] = float("nan") if kind == "scale_nan" else 0.0
+    elif kind == "value_nan":
+        state["gate_up_q"].view(torch.uint8)[0, 0, 0] = 0xFF
+    else:
+        state = packed(c=192)
+    with pytest.raises(ValueError):
+        pkg().B200FP8RoutedExperts.from_packed(state)
+
+
+def test_bank_is_inference_only_and_keeps_its_types():
+    bank = pkg().B200FP8RoutedExperts.from_packed(packed())
+    assert bank.to("cpu") is bank and not bank.training
+    with pytest.raises(TypeError, match="casts"):
+        bank.to(BF16)
+    with pytest.raises(RuntimeError, match="inference"):
+        bank.train()
+    x, top, gate = torch.ones(3, 128, dtype=BF16), torch.zeros(3, 1, dtype=torch.int64), torch.ones(3, 1, dtype=BF16)
+    with pytest.raises(ValueError, match="CUDA"):
+        bank.routed_forward(x, top, gate, scaling=1.0, chunk_size=2)
+    with pytest.raises(RuntimeError, match="inference"):
+        bank.routed_forward(x.requires_grad_(), top, gate, scaling=1.0, chunk_size=2)
+    for kw in (dict(scaling=float("nan"), chunk_size=2), dict(scaling=1.0, chunk_size=0)):
+        with pytest.raises(ValueError):
+            bank.routed_forward(x.detach(), top, gate, **kw)
+    assert set(bank.state_dict()) == set(packed())
+    again = pkg().B200FP8RoutedExperts.from_packed({k: v.clone() for k, v in bank.state_dict().items()})
+    assert (again.num_experts, again.in_features, again.hidden_features) == (2, 128, 128)
+
+
+def test_module_takes_groups_and_formats():
+    M = pkg().B200MoEFeedForward
+    m = M(128, 128, 16, 4, router_groups=4, router_top_groups=2)
+    assert (m.router_groups, m.router_top_groups, m.router_group_score) == (4, 2, "top2")
+    for kw in (dict(router_groups=3, router_top_groups=1), dict(router_groups=4), dict(router_top_groups=2),
+               dict(router_groups=8, router_top_groups=1), dict(router_group_score="mean")):
+        with pytest.raises(ValueError):
+            M(128, 128, 16, 4, **kw)
+    with pytest.raises(ValueError, match="format"):
+        m.set_routed_weights(torch.zeros(16, 128, 256, dtype=BF16), torch.zeros(16, 128, 128, dtype=BF16), "int8")
+    with pytest.raises(ValueError, match="shared"):
+        M(128, 128, 16, 4, shared_expert=False).quantize_shared()
+
+
+def test_fake_shapes_of_the_torch_operators():
+    pkg()
+    t, c, e, k, f = 10, 256, 8, 2, 128
+    with FakeTensorMode():
+        x = cuda(t, c)
+        top, gate = torch.ops.praxis_b200.route_groups(cuda(t, e, dtype=torch.float32), None, k, "sigmoid", 4, 2, "max")
+        assert (top.shape, top.dtype, gate.shape, gate.dtype) == ((t, k), torch.int64, (t, k), BF16)
+        y = torch.ops.praxis_b200.fp8_linear(cuda(2, 5, c), *weight(300, c))
+        assert (y.shape, y.dtype) == ((2, 5, 300), BF16)
+        assert torch.ops.praxis_b200.fp8_mlp(x, *weight(2 * f, c), *weight(c, f)).shape == (t, c)
+        y = torch.ops.praxis_b200.fp8_moe_forward(x, top, gate, *weight(e, 2 * f, c), *weight(e, c, f), 2.5, None)
+        assert (y.shape, y.dtype) == ((t, c), BF16)

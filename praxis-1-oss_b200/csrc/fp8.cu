@@ -147,11 +147,12 @@ __global__ void __launch_bounds__(256) fp8_pack_kernel(const uint16_t* __restric
 // warp 1      MMA issuer (leader CTA): per k-block two MMA groups of 128
 //             columns ("halves"), each into one of its two tensor-memory
 //             buffers: 4 x 128 columns are all 512
-// warps 2..9  epilogue: half h = (warp - 2) / 4 belongs to four warps, one per
+// warps 4..11 epilogue: half h = (warp - 4) / 4 belongs to four warps, one per
 //             lane quadrant. Per k-block a thread reads the 128 columns of its
-//             row and adds them, times sx * sw, to 128 registers. A buffer is
-//             free again as soon as it is read, 3 MMA groups (768 clocks)
-//             before the issuer needs it.
+//             row in four loads, the next in flight while it adds the last,
+//             times sx * sw, to 128 registers. A buffer is free again as soon
+//             as it is read, 3 MMA groups (768 clocks) before the issuer needs
+//             it.
 //
 // Bound: 128 x 256 x 128 products are 512 clocks of one SM's tensor core; the
 // FMAs of the 128 x 256 block sums are 256 clocks of its fp32 lanes.
@@ -186,7 +187,13 @@ struct Fp8Shape {
   static constexpr int STAGES = CTAS == 2 ? 6 : 4;
   static constexpr int EPI_WARPS = 8;
   static constexpr int OUT_BOX = 4096;  // 32 rows x 64 bf16 per epilogue warp
-  static constexpr int THREADS = 32 * (2 + EPI_WARPS);
+  // Registers: 12 warps launch with 168 each (64512 in all); the four warps
+  // of the producer and the issuer give some back, and the epilogue's 128
+  // sums and two 32-column loads in flight fit without spilling.
+  static constexpr int EPI_WARP0 = 4;
+  static constexpr int THREADS = 32 * (EPI_WARP0 + EPI_WARPS);
+  static constexpr int LAUNCH_REGS = 168, FRONT_REGS = 40, EPI_REGS = 232;
+  static_assert(32 * EPI_WARP0 * FRONT_REGS + 32 * EPI_WARPS * EPI_REGS <= THREADS * LAUNCH_REGS, "register split");
   static constexpr size_t SMEM_BYTES = 1024 + (size_t)STAGES * STAGE_BYTES + EPI_WARPS * OUT_BOX + 256;
   static_assert(SMEM_BYTES <= 232448, "shared memory budget");
 };
@@ -219,6 +226,30 @@ template <int CTAS>
 __device__ __forceinline__ void fp8_commit(uint64_t* bar) {
   if constexpr (CTAS == 1) tc_commit(bar);
   else tc_commit_pair(bar, 0x3);
+}
+
+// acc[0..7] += f * (the 16 columns in r), one FMA each. The statements are
+// volatile, so they stay behind the wait for the loads of r.
+__device__ __forceinline__ void fp8_add_block(uint64_t* acc, const uint32_t (&r)[16], float f) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    asm volatile(
+        "{\n\t.reg .b64 d, s;\n\tmov.b64 d, {%1, %2};\n\tmov.b64 s, {%3, %3};\n\t"
+        "fma.rn.f32x2 %0, d, s, %0;\n\t}"
+        : "+l"(acc[j])
+        : "r"(r[2 * j]), "r"(r[2 * j + 1]), "f"(f));
+}
+__device__ __forceinline__ float2 unpack_f32x2(uint64_t v) {
+  return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
+}
+
+template <int REGS>
+__device__ __forceinline__ void regs_up() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS));
+}
+template <int REGS>
+__device__ __forceinline__ void regs_down() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS));
 }
 
 // Row tile m of the launch: dense rows, or the table's entry.
@@ -301,8 +332,9 @@ __device__ __forceinline__ void fp8_gemm_body(const Fp8GemmParams& p) {
   const int k_blocks = (p.K + kFp8Block - 1) / kFp8Block;
   const int first = blockIdx.x / CTAS, step = gridDim.x / CTAS;
 
-  if (warp == 0) {
-    if (lane == 0) {
+  if (warp < S::EPI_WARP0) {
+    regs_down<S::FRONT_REGS>();
+    if (warp == 0 && lane == 0) {
       // ---------------- TMA producer (every CTA) ----------------
       const uint32_t full_leader = CTAS == 1 ? 0u : mapa_shared(smem_u32(full), 0);
       uint32_t stage = 0, phase = 0;
@@ -346,9 +378,7 @@ __device__ __forceinline__ void fp8_gemm_body(const Fp8GemmParams& p) {
       if (!ok && rank == 0)
         for (uint32_t s = 0; s < S::STAGES; ++s)
           mbar_wait(&full[s], s < stage ? phase : phase ^ 1u, kErrTimeoutProducer, 50000000ull, false);
-    }
-  } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
+    } else if (warp == 1 && lane == 0 && rank == 0) {
       // ---------------- MMA issuer (leader) ----------------
       constexpr uint32_t idesc = idesc_e4m3(128 * CTAS, 128);
       uint32_t stage = 0, phase = 0, cnt = 0;
@@ -381,15 +411,16 @@ __device__ __forceinline__ void fp8_gemm_body(const Fp8GemmParams& p) {
       }
     }
   } else {
-    // ---------------- epilogue (warps 2..9, every CTA) ----------------
+    regs_up<S::EPI_REGS>();
+    // ---------------- epilogue (warps 4..11, every CTA) ----------------
     // After a wait that gave up the warps go through the remaining units
     // without waiting or storing, so that the named barriers stay matched.
     const uint32_t quad = (uint32_t)(warp & 3);
-    const int h = (warp - 2) >> 2;
+    const int h = (warp - S::EPI_WARP0) >> 2;
     const int row_in_cta = (int)(quad * 32 + lane);
     const uint32_t acc_empty_leader = CTAS == 1 ? 0u : mapa_shared(smem_u32(acc_empty), 0);
     const uint32_t taddr = tmem + ((quad * 32u) << 16) + 256u * h;
-    uint8_t* box = sOut + (warp - 2) * S::OUT_BOX;
+    uint8_t* box = sOut + (warp - S::EPI_WARP0) * S::OUT_BOX;
     const int n_blocks = (p.N + kFp8Block - 1) / kFp8Block;
     uint32_t cnt = 0, unit = 0;
     bool ok = true;
@@ -405,50 +436,60 @@ __device__ __forceinline__ void fp8_gemm_body(const Fp8GemmParams& p) {
       const int nb1 = MODE == FP8_SWIGLU ? n + F / 128 : nb0;
       const float* ws0 = p.ws + ((int64_t)t.expert * n_blocks + nb0) * k_blocks;
       const float* ws1 = p.ws + ((int64_t)t.expert * n_blocks + nb1) * k_blocks;
-      float2 acc[64];
+      uint64_t acc[64];  // two neighbouring columns each
 #pragma unroll
-      for (int j = 0; j < 64; ++j) acc[j] = make_float2(0.0f, 0.0f);
-      float sx = __ldg(xs), w0 = __ldg(ws0), w1 = __ldg(ws1);
+      for (int j = 0; j < 64; ++j) acc[j] = 0;
+      float f0 = __ldg(xs) * __ldg(ws0), f1 = MODE == FP8_SWIGLU ? __ldg(xs) * __ldg(ws1) : f0;
+      uint32_t ra[16], rb[16];
+      ok = ok && mbar_wait(&acc_full[2 * h + (cnt & 1u)], (cnt >> 1) & 1u, kErrTimeoutEpilogue);
+      tc_fence_after();
+      tc_ld_32x32b_x16(taddr + (cnt & 1u) * 128, ra);
       for (int kb = 0; kb < k_blocks; ++kb, ++cnt) {
-        const uint32_t buf = cnt & 1u;
-        const float f0 = sx * w0, f1 = sx * w1;
+        const uint32_t buf = cnt & 1u, tb = taddr + buf * 128;
+        float sx = 0.0f, w0 = 0.0f, w1 = 0.0f;
         if (kb + 1 < k_blocks) {
           sx = __ldg(xs + (int64_t)(kb + 1) * p.xs_ld);
           w0 = __ldg(ws0 + kb + 1);
-          w1 = __ldg(ws1 + kb + 1);
+          if (MODE == FP8_SWIGLU) w1 = __ldg(ws1 + kb + 1);
         }
-        ok = ok && mbar_wait(&acc_full[2 * h + buf], (cnt >> 1) & 1u, kErrTimeoutEpilogue);
-        tc_fence_after();
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t r[32];
-          tc_ld_32x32b_x32(taddr + buf * 128 + c * 32, r);
+        for (int c = 0; c < 8; c += 2) {
+          const float f = c < 4 ? f0 : f1;
           tc_wait_ld();
-          if (c == 3) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) {
-              if (CTAS == 1 || rank == 0) mbar_arrive(&acc_empty[2 * h + buf]);
-              else mbar_arrive_cluster(acc_empty_leader + (2 * h + buf) * 8);
-            }
-          }
-          const float f = (MODE == FP8_SWIGLU && c >= 2) ? f1 : f0;
-          const float2 ff = make_float2(f, f);
-#pragma unroll
-          for (int j = 0; j < 16; ++j)
-            acc[c * 16 + j] =
-                fma2_rn(make_float2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])), ff, acc[c * 16 + j]);
+          tc_ld_32x32b_x16(tb + 16 * (c + 1), rb);
+          fp8_add_block(acc + 8 * c, ra, f);
+          if (c == 6) break;
+          tc_wait_ld();
+          tc_ld_32x32b_x16(tb + 16 * (c + 2), ra);
+          fp8_add_block(acc + 8 * (c + 1), rb, f);
         }
+        tc_wait_ld();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (CTAS == 1 || rank == 0) mbar_arrive(&acc_empty[2 * h + buf]);
+          else mbar_arrive_cluster(acc_empty_leader + (2 * h + buf) * 8);
+        }
+        if (kb + 1 < k_blocks) {
+          const uint32_t next = cnt + 1;
+          ok = ok && mbar_wait(&acc_full[2 * h + (next & 1u)], (next >> 1) & 1u, kErrTimeoutEpilogue);
+          tc_fence_after();
+          tc_ld_32x32b_x16(taddr + (next & 1u) * 128, ra);
+        }
+        fp8_add_block(acc + 56, rb, f1);
+        f0 = sx * w0;
+        f1 = MODE == FP8_SWIGLU ? sx * w1 : f0;
       }
       if constexpr (MODE == FP8_SWIGLU) {
         // 64 hidden columns 128 n + 64 h ..; the other half's warps hold the
         // rest of the row's block, so the row maxima meet in shared memory
         float a = kFp8MinAmax;
+        float2 hid[32];
 #pragma unroll
         for (int j = 0; j < 32; ++j) {
-          acc[j].x = swiglu_f32(acc[j].x, acc[32 + j].x);
-          acc[j].y = swiglu_f32(acc[j].y, acc[32 + j].y);
-          a = fmaxf(a, fmaxf(fabsf(acc[j].x), fabsf(acc[j].y)));
+          const float2 g = unpack_f32x2(acc[j]), v = unpack_f32x2(acc[32 + j]);
+          hid[j] = make_float2(swiglu_f32(g.x, v.x), swiglu_f32(g.y, v.y));
+          a = fmaxf(a, fmaxf(fabsf(hid[j].x), fabsf(hid[j].y)));
         }
         float* s_max = reinterpret_cast<float*>(sOut) + (unit & 1u) * 256;
         s_max[h * 128 + row_in_cta] = a;
@@ -462,7 +503,7 @@ __device__ __forceinline__ void fp8_gemm_body(const Fp8GemmParams& p) {
             uint32_t c[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const float2 v0 = acc[8 * j + 2 * i], v1 = acc[8 * j + 2 * i + 1];
+              const float2 v0 = hid[8 * j + 2 * i], v1 = hid[8 * j + 2 * i + 1];
               c[i] = cvt_e4m3x4(mul_rn(v0.x, r), mul_rn(v0.y, r), mul_rn(v1.x, r), mul_rn(v1.y, r));
             }
             dst[j] = make_uint4(c[0], c[1], c[2], c[3]);
@@ -481,10 +522,14 @@ __device__ __forceinline__ void fp8_gemm_body(const Fp8GemmParams& p) {
             __syncwarp();
 #pragma unroll
             for (int c = 0; c < 8; ++c) {
-              const float2* v = acc + i * 32 + c * 4;
+              uint32_t w[4];
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const float2 v = unpack_f32x2(acc[i * 32 + c * 4 + j]);
+                w[j] = cvt_bf16x2(v.x, v.y);
+              }
               *reinterpret_cast<uint4*>(box + lane * 128 + ((c ^ (lane & 7)) << 4)) =
-                  make_uint4(cvt_bf16x2(v[0].x, v[0].y), cvt_bf16x2(v[1].x, v[1].y), cvt_bf16x2(v[2].x, v[2].y),
-                             cvt_bf16x2(v[3].x, v[3].y));
+                  make_uint4(w[0], w[1], w[2], w[3]);
             }
             fence_proxy_async_shared();
             __syncwarp();
@@ -498,8 +543,9 @@ __device__ __forceinline__ void fp8_gemm_body(const Fp8GemmParams& p) {
           uint16_t* dst = p.out + row * p.N + col0;
 #pragma unroll
           for (int j = 0; j < 64; ++j) {
-            if (col0 + 2 * j < p.N) dst[2 * j] = f32_to_bf16(acc[j].x);
-            if (col0 + 2 * j + 1 < p.N) dst[2 * j + 1] = f32_to_bf16(acc[j].y);
+            const float2 v = unpack_f32x2(acc[j]);
+            if (col0 + 2 * j < p.N) dst[2 * j] = f32_to_bf16(v.x);
+            if (col0 + 2 * j + 1 < p.N) dst[2 * j + 1] = f32_to_bf16(v.y);
           }
         }
       }
@@ -560,6 +606,12 @@ static int fp8_launch(const Fp8GemmParams& p, int64_t units, cudaStream_t stream
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM_BYTES);
     if (e != cudaSuccess)
       return set_error(PRAXIS_B200_ECUDA, "fp8 gemm smem attribute (device %d): %s", dev, cudaGetErrorString(e));
+    // setmaxnreg waits for registers that the launch does not have
+    cudaFuncAttributes fa;
+    e = cudaFuncGetAttributes(&fa, kernel);
+    if (e != cudaSuccess || fa.numRegs < S::LAUNCH_REGS)
+      return set_error(PRAXIS_B200_ECUDA, "fp8 gemm: built with %d registers a thread, needs %d", fa.numRegs,
+                       S::LAUNCH_REGS);
     int n = sm_count();
     if (CTAS == 2) {
       cudaLaunchConfig_t cfg = {};

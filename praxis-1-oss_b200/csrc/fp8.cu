@@ -161,7 +161,7 @@ enum Fp8Mode : int { FP8_PLAIN = 0, FP8_SWIGLU = 1 };
 
 struct Fp8GemmParams {
   CUtensorMap tmap_a;    // activation codes [rows, K], boxes of 128 rows
-  CUtensorMap tmap_b;    // weight codes [E * N, K], boxes of 64 rows
+  CUtensorMap tmap_b;    // weight codes [E * N, K], boxes of 128 rows
   CUtensorMap tmap_out;  // bf16 output [rows, N], boxes of 32 rows x 64 columns (FP8_PLAIN, N % 8 == 0)
   const float* xs;       // activation scales, [K blocks][xs_ld]
   int64_t xs_ld;
@@ -205,20 +205,24 @@ __host__ __device__ constexpr uint32_t idesc_e4m3(uint32_t m, uint32_t n) {
          | ((m >> 4) << 24);  // M / 16
 }
 
-template <int CTAS>
-__device__ __forceinline__ void tc_mma_e4m3(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
-                                            uint32_t accumulate) {
+// The high word of a descriptor is the same for every operand here; the low
+// word (the address) moves by 2 per 32 bytes.
+template <int CTAS, int ACCUMULATE>
+__device__ __forceinline__ void tc_mma_e4m3(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t desc_hi,
+                                            uint32_t idesc) {
   if constexpr (CTAS == 1)
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %5, 0;\n\t"
+        "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %4, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_lo), "r"(b_lo), "r"(desc_hi), "r"(idesc), "n"(ACCUMULATE)
         : "memory");
   else
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %5, 0;\n\t"
+        "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], a, b, %4, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_lo), "r"(b_lo), "r"(desc_hi), "r"(idesc), "n"(ACCUMULATE)
         : "memory");
 }
 
@@ -241,6 +245,27 @@ __device__ __forceinline__ void fp8_add_block(uint64_t* acc, const uint32_t (&r)
 }
 __device__ __forceinline__ float2 unpack_f32x2(uint64_t v) {
   return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
+}
+
+// mbar_wait (common.cuh) that looks at the clock only every 64 tries: a wait
+// per k-block and role is on the path of every MMA here, and the first read of
+// %globaltimer alone costs about as much as a k-block's products.
+__device__ __forceinline__ bool fp8_wait(uint64_t* bar, uint32_t parity, unsigned int code,
+                                         uint64_t limit_ns = 2000000000ull, bool stop_on_error = true) {
+  uint64_t start = 0;
+  for (uint32_t i = 1;; ++i) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((i & 63u) == 0u) {
+      if (stop_on_error && error_raised()) return false;
+      const uint64_t now = globaltimer_ns();
+      if (start == 0) {
+        start = now;
+      } else if (now - start > limit_ns) {
+        record_error(code);
+        return false;
+      }
+    }
+  }
 }
 
 template <int REGS>
@@ -273,6 +298,12 @@ __device__ __forceinline__ float swiglu_f32(float g, float u) {
   return __fdividef(1.0f, 1.0f + __expf(-g)) * g * u;
 }
 
+// Tensor-memory column of a thread's chunk c of 16 columns, from its first.
+template <int MODE>
+__device__ constexpr uint32_t chunk_col(int c) {
+  return 16 * c + (MODE == FP8_SWIGLU && c >= 4 ? 64 : 0);
+}
+
 template <int CTAS, int MODE>
 __device__ __forceinline__ void fp8_gemm_body(const Fp8GemmParams& p) {
   pdl_wait();  // the previous kernel of the stream has completed
@@ -285,9 +316,9 @@ __device__ __forceinline__ void fp8_gemm_body(const Fp8GemmParams& p) {
   uint8_t* sOut = sB + S::STAGES * S::B_BYTES;  // output boxes; FP8_SWIGLU: row maxima [2 units][2 halves][128]
   uint64_t* full = reinterpret_cast<uint64_t*>(sOut + S::EPI_WARPS * S::OUT_BOX);
   uint64_t* empty = full + S::STAGES;
-  uint64_t* acc_full = empty + S::STAGES;  // [half][buffer]
-  uint64_t* acc_empty = acc_full + 4;      // [half][buffer], the leader's
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 4);
+  uint64_t* acc_full = empty + S::STAGES;  // per buffer
+  uint64_t* acc_empty = acc_full + 2;      // per buffer, the leader's
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
 
   const int warp = threadIdx.x >> 5;
   const uint32_t lane = threadIdx.x & 31;
@@ -298,9 +329,9 @@ __device__ __forceinline__ void fp8_gemm_body(const Fp8GemmParams& p) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
-    for (int b = 0; b < 4; ++b) {
+    for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], 4 * CTAS);
+      mbar_init(&acc_empty[b], S::EPI_WARPS * CTAS);
     }
     fence_barrier_init();
   }
@@ -343,15 +374,11 @@ __device__ __forceinline__ void fp8_gemm_body(const Fp8GemmParams& p) {
         const int m = u / n_tiles, n = u - m * n_tiles;
         const TileEntry t = fp8_tile<CTAS>(p, m);
         const int a_row = t.row0 + 128 * (int)rank;
-        // weight row of box i: half h, 64-row part (the pair's part is its rank)
-        int b_row[4 / CTAS];
-#pragma unroll
-        for (int i = 0; i < 4 / CTAS; ++i) {
-          const int h = CTAS == 1 ? i >> 1 : i, part = CTAS == 1 ? i & 1 : (int)rank;
-          b_row[i] = t.expert * p.N + (MODE == FP8_SWIGLU ? part * F + n * 128 + 64 * h : n * 256 + 128 * h + 64 * part);
-        }
+        // the weight rows of columns 0..127 (leader) and 128..255 (its peer)
+        const int b_row = t.expert * p.N + (MODE == FP8_SWIGLU ? n * 128 : n * 256);
+        const int b_up = MODE == FP8_SWIGLU ? F : 128;
         for (int kb = 0; kb < k_blocks; ++kb) {
-          if (!mbar_wait(&empty[stage], phase ^ 1u, kErrTimeoutProducer)) {
+          if (!fp8_wait(&empty[stage], phase ^ 1u, kErrTimeoutProducer)) {
             ok = false;
             break;
           }
@@ -360,13 +387,12 @@ __device__ __forceinline__ void fp8_gemm_body(const Fp8GemmParams& p) {
           uint8_t* b = sB + stage * S::B_BYTES;
           if constexpr (CTAS == 1) {
             tma_load_2d(a, &p.tmap_a, &full[stage], kb * 128, a_row);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) tma_load_2d(b + i * 8192, &p.tmap_b, &full[stage], kb * 128, b_row[i]);
+            tma_load_2d(b, &p.tmap_b, &full[stage], kb * 128, b_row);
+            tma_load_2d(b + 16384, &p.tmap_b, &full[stage], kb * 128, b_row + b_up);
           } else {
             const uint32_t fb = full_leader + stage * 8;
             tma_load_2d_pair(a, &p.tmap_a, fb, kb * 128, a_row);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) tma_load_2d_pair(b + i * 8192, &p.tmap_b, fb, kb * 128, b_row[i]);
+            tma_load_2d_pair(b, &p.tmap_b, fb, kb * 128, b_row + (int)rank * b_up);
           }
           if (++stage == S::STAGES) {
             stage = 0;
@@ -377,31 +403,30 @@ __device__ __forceinline__ void fp8_gemm_body(const Fp8GemmParams& p) {
       // after an error the copies in flight still land before the CTA ends
       if (!ok && rank == 0)
         for (uint32_t s = 0; s < S::STAGES; ++s)
-          mbar_wait(&full[s], s < stage ? phase : phase ^ 1u, kErrTimeoutProducer, 50000000ull, false);
+          fp8_wait(&full[s], s < stage ? phase : phase ^ 1u, kErrTimeoutProducer, 50000000ull, false);
     } else if (warp == 1 && lane == 0 && rank == 0) {
       // ---------------- MMA issuer (leader) ----------------
-      constexpr uint32_t idesc = idesc_e4m3(128 * CTAS, 128);
+      constexpr uint32_t idesc = idesc_e4m3(128 * CTAS, 256);
+      const uint64_t a_desc = smem_desc(smem_u32(sA), 16, 1024, kLayoutSwizzle128B);
+      const uint32_t desc_hi = (uint32_t)(a_desc >> 32), a_lo = (uint32_t)a_desc;
+      const uint32_t b_lo = (uint32_t)smem_desc(smem_u32(sB), 16, 1024, kLayoutSwizzle128B);
       uint32_t stage = 0, phase = 0, cnt = 0;
       bool ok = true;
       for (int u = first; u < total && ok; u += step) {
         for (int kb = 0; kb < k_blocks && ok; ++kb, ++cnt) {
           const uint32_t buf = cnt & 1u, buf_phase = (cnt >> 1) & 1u;
-          ok = mbar_wait(&full[stage], phase, kErrTimeoutMma);
+          ok = fp8_wait(&full[stage], phase, kErrTimeoutMma);
           if (!ok) break;
-          const uint32_t a = smem_u32(sA + stage * S::A_BYTES), b = smem_u32(sB + stage * S::B_BYTES);
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            ok = mbar_wait(&acc_empty[2 * h + buf], buf_phase ^ 1u, kErrTimeoutMma);
-            if (!ok) break;
-            tc_fence_after();
-#pragma unroll
-            for (int ks = 0; ks < 4; ++ks)
-              tc_mma_e4m3<CTAS>(tmem + (2 * h + buf) * 128, smem_desc(a + ks * 32, 16, 1024, kLayoutSwizzle128B),
-                                smem_desc(b + h * (16384 / CTAS) + ks * 32, 16, 1024, kLayoutSwizzle128B), idesc,
-                                ks != 0 ? 1u : 0u);
-            fp8_commit<CTAS>(&acc_full[2 * h + buf]);
-          }
+          const uint32_t a = a_lo + stage * (S::A_BYTES >> 4), b = b_lo + stage * (S::B_BYTES >> 4);
+          ok = fp8_wait(&acc_empty[buf], buf_phase ^ 1u, kErrTimeoutMma);
           if (!ok) break;
+          tc_fence_after();
+          const uint32_t d = tmem + buf * 256;
+          tc_mma_e4m3<CTAS, 0>(d, a, b, desc_hi, idesc);
+          tc_mma_e4m3<CTAS, 1>(d, a + 2, b + 2, desc_hi, idesc);
+          tc_mma_e4m3<CTAS, 1>(d, a + 4, b + 4, desc_hi, idesc);
+          tc_mma_e4m3<CTAS, 1>(d, a + 6, b + 6, desc_hi, idesc);
+          fp8_commit<CTAS>(&acc_full[buf]);
           fp8_commit<CTAS>(&empty[stage]);
           if (++stage == S::STAGES) {
             stage = 0;
@@ -419,7 +444,8 @@ __device__ __forceinline__ void fp8_gemm_body(const Fp8GemmParams& p) {
     const int h = (warp - S::EPI_WARP0) >> 2;
     const int row_in_cta = (int)(quad * 32 + lane);
     const uint32_t acc_empty_leader = CTAS == 1 ? 0u : mapa_shared(smem_u32(acc_empty), 0);
-    const uint32_t taddr = tmem + ((quad * 32u) << 16) + 256u * h;
+    // SwiGLU: 64 gate columns and the up columns 128 further on; else 128 in a row
+    const uint32_t taddr = tmem + ((quad * 32u) << 16) + (MODE == FP8_SWIGLU ? 64u : 128u) * h;
     uint8_t* box = sOut + (warp - S::EPI_WARP0) * S::OUT_BOX;
     const int n_blocks = (p.N + kFp8Block - 1) / kFp8Block;
     uint32_t cnt = 0, unit = 0;
@@ -441,11 +467,11 @@ __device__ __forceinline__ void fp8_gemm_body(const Fp8GemmParams& p) {
       for (int j = 0; j < 64; ++j) acc[j] = 0;
       float f0 = __ldg(xs) * __ldg(ws0), f1 = MODE == FP8_SWIGLU ? __ldg(xs) * __ldg(ws1) : f0;
       uint32_t ra[16], rb[16];
-      ok = ok && mbar_wait(&acc_full[2 * h + (cnt & 1u)], (cnt >> 1) & 1u, kErrTimeoutEpilogue);
+      ok = ok && fp8_wait(&acc_full[cnt & 1u], (cnt >> 1) & 1u, kErrTimeoutEpilogue);
       tc_fence_after();
-      tc_ld_32x32b_x16(taddr + (cnt & 1u) * 128, ra);
+      tc_ld_32x32b_x16(taddr + (cnt & 1u) * 256, ra);
       for (int kb = 0; kb < k_blocks; ++kb, ++cnt) {
-        const uint32_t buf = cnt & 1u, tb = taddr + buf * 128;
+        const uint32_t buf = cnt & 1u, tb = taddr + buf * 256;
         float sx = 0.0f, w0 = 0.0f, w1 = 0.0f;
         if (kb + 1 < k_blocks) {
           sx = __ldg(xs + (int64_t)(kb + 1) * p.xs_ld);
@@ -456,25 +482,25 @@ __device__ __forceinline__ void fp8_gemm_body(const Fp8GemmParams& p) {
         for (int c = 0; c < 8; c += 2) {
           const float f = c < 4 ? f0 : f1;
           tc_wait_ld();
-          tc_ld_32x32b_x16(tb + 16 * (c + 1), rb);
+          tc_ld_32x32b_x16(tb + chunk_col<MODE>(c + 1), rb);
           fp8_add_block(acc + 8 * c, ra, f);
           if (c == 6) break;
           tc_wait_ld();
-          tc_ld_32x32b_x16(tb + 16 * (c + 2), ra);
+          tc_ld_32x32b_x16(tb + chunk_col<MODE>(c + 2), ra);
           fp8_add_block(acc + 8 * (c + 1), rb, f);
         }
         tc_wait_ld();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) {
-          if (CTAS == 1 || rank == 0) mbar_arrive(&acc_empty[2 * h + buf]);
-          else mbar_arrive_cluster(acc_empty_leader + (2 * h + buf) * 8);
+          if (CTAS == 1 || rank == 0) mbar_arrive(&acc_empty[buf]);
+          else mbar_arrive_cluster(acc_empty_leader + buf * 8);
         }
         if (kb + 1 < k_blocks) {
           const uint32_t next = cnt + 1;
-          ok = ok && mbar_wait(&acc_full[2 * h + (next & 1u)], (next >> 1) & 1u, kErrTimeoutEpilogue);
+          ok = ok && fp8_wait(&acc_full[next & 1u], (next >> 1) & 1u, kErrTimeoutEpilogue);
           tc_fence_after();
-          tc_ld_32x32b_x16(taddr + (next & 1u) * 128, ra);
+          tc_ld_32x32b_x16(taddr + (next & 1u) * 256, ra);
         }
         fp8_add_block(acc + 56, rb, f1);
         f0 = sx * w0;
@@ -687,7 +713,7 @@ int run_fp8_gemm(const Fp8Gemm& g, cudaStream_t stream) {
   memset(&p, 0, sizeof(p));
   int rc = fp8_map(&p.tmap_a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, g.q, g.rows, g.k, 128, 128);
   if (rc) return rc;
-  rc = fp8_map(&p.tmap_b, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, g.wq, (int64_t)g.experts * g.n, g.k, 128, 64);
+  rc = fp8_map(&p.tmap_b, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, g.wq, (int64_t)g.experts * g.n, g.k, 128, 128);
   if (rc) return rc;
   const bool swiglu = g.out == nullptr;
   if (!swiglu && g.n % 8 == 0 && ((uintptr_t)g.out & 15) == 0) {

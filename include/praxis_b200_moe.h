@@ -449,7 +449,7 @@ int praxis_b200_fp8_linear(const void* x, int64_t rows, int32_t k, int64_t ldx, 
  * [E, C/128, F/128]; dense: E = 1. Routed: the dispatch and the combine of
  * praxis_b200_moe_forward (out[t] = bf16(sum of gate * scaling * y), then
  * bf16(out + shared)). Dense: out = y; gate, scaling and shared are not used.
- * C and F multiples of 128, buffers 16-byte aligned. */
+ * C and F multiples of 128, buffers 16-byte, the workspace 32-byte aligned. */
 typedef struct praxis_b200_fp8_ffn_args {
   const void* x;              /* [T, C] bf16 */
   const int64_t* top_idx;     /* [T, k] */

@@ -719,7 +719,7 @@ int praxis_b200_fp8_quantize(const void* x, int64_t rows, int32_t cols, int64_t 
   if (!x || !q || !scale) return set_error(PRAXIS_B200_EINVAL, "fp8_quantize: null pointer");
   if (ldx < cols || ldx % 8 != 0 || scale_ld < rows || (((uintptr_t)x | (uintptr_t)q) & 15))
     return set_error(PRAXIS_B200_EINVAL, "fp8_quantize: row pitch or alignment");
-  return run_fp8_quantize(static_cast<const uint16_t*>(x), rows, cols, ldx, Fp8Rows{}, static_cast<uint8_t*>(q), scale,
+  return run_fp8_quantize(static_cast<const uint16_t*>(x), rows, cols, ldx, kFp8SameRows, static_cast<uint8_t*>(q), scale,
                           scale_ld, PRAXIS_STREAM(stream));
 }
 
@@ -754,7 +754,7 @@ int praxis_b200_fp8_linear(const void* x, int64_t rows, int32_t k, int64_t ldx, 
   cudaStream_t s = PRAXIS_STREAM(stream);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   float* scale = reinterpret_cast<float*>(ws + L.scale);
-  rc = run_fp8_quantize(static_cast<const uint16_t*>(x), rows, k, ldx, Fp8Rows{}, ws + L.q, scale, L.scale_ld, s);
+  rc = run_fp8_quantize(static_cast<const uint16_t*>(x), rows, k, ldx, kFp8SameRows, ws + L.q, scale, L.scale_ld, s);
   if (rc) return rc;
   Fp8Gemm g = {};
   g.q = ws + L.q;
@@ -796,9 +796,9 @@ int praxis_b200_fp8_ffn(const praxis_b200_fp8_ffn_args* a) {
   if (!a->x || (!a->out && !a->tail) || !a->gate_up_q || !a->gate_up_scale || !a->down_q || !a->down_scale ||
       !a->workspace || (routed && (!a->top_idx || !a->gate)))
     return set_error(PRAXIS_B200_EINVAL, "fp8_ffn: null pointer");
-  if (((uintptr_t)a->x | (uintptr_t)a->out | (uintptr_t)a->gate_up_q | (uintptr_t)a->down_q | (uintptr_t)a->shared |
-       (uintptr_t)a->workspace) & 15)
-    return set_error(PRAXIS_B200_EINVAL, "fp8_ffn: buffers must be 16-byte aligned");
+  if ((((uintptr_t)a->x | (uintptr_t)a->out | (uintptr_t)a->gate_up_q | (uintptr_t)a->down_q | (uintptr_t)a->shared) & 15) ||
+      ((uintptr_t)a->workspace & 31))
+    return set_error(PRAXIS_B200_EINVAL, "fp8_ffn: buffers must be 16-byte, the workspace 32-byte aligned");
   if (a->workspace_size < L.total)
     return set_error(PRAXIS_B200_EINVAL, "fp8_ffn: workspace %zu < %zu bytes", a->workspace_size, L.total);
   cudaStream_t s = PRAXIS_STREAM(a->stream);
@@ -811,7 +811,7 @@ int praxis_b200_fp8_ffn(const praxis_b200_fp8_ffn_args* a) {
   float* as = reinterpret_cast<float*>(ws + L.as);
   float* hs = reinterpret_cast<float*>(ws + L.hs);
   uint16_t* rows = routed ? reinterpret_cast<uint16_t*>(ws + L.rows) : static_cast<uint16_t*>(a->out);
-  Fp8Rows to = {};
+  Fp8Rows to = kFp8SameRows;
   if (routed) {
     rc = run_dispatch(a->top_idx, static_cast<const uint16_t*>(a->gate), nullptr, a->tokens, top_k, a->experts,
                       Passes{1, 0}, ws + L.dispatch, L.inverse - L.dispatch, nullptr, inverse, nullptr, nullptr,

@@ -35,63 +35,70 @@ __device__ __forceinline__ uint32_t cvt_e4m3x4(float a, float b, float c, float 
 // ---------------------------------------------------------------------------
 // Activation quantization
 // ---------------------------------------------------------------------------
-// Sixteen lanes take one block of 128 columns (8 columns, 16 bytes, each): the
-// largest magnitude is four shuffles, and a warp reads 512 and writes 256
-// contiguous bytes. Scales are stored block-major, scale[b * scale_ld + row]:
-// the GEMM epilogue reads one block's scales of 32 consecutive rows at once.
-// With `inverse` the block goes to the rows of the token's K routed slots
-// (pcsr[e] + inverse - csr[e], as the dispatch laid them out), quantized once.
+// A warp takes 1024 columns of a row, four 16-byte loads per lane in flight;
+// sixteen lanes hold one block of 128 columns, whose largest magnitude is four
+// shuffles. Scales are stored block-major, scale[b * scale_ld + row]: the GEMM
+// epilogue reads one block's scales of 32 consecutive rows at once. With
+// `top_idx` the row goes to the rows of the token's routed slots (pcsr[e] +
+// inverse - csr[e], as the dispatch laid them out), quantized once.
 struct Fp8Rows {
   const int64_t* top_idx;  // [rows, top_k]; nullptr: row r goes to row r
   const int64_t* inverse;
   const int32_t* csr;
   const int32_t* pcsr;
-  int32_t top_k;
+  int32_t top_k;  // 1 without top_idx
   int32_t experts;
 };
 
-constexpr int kFp8QuantThreads = 256;
+constexpr Fp8Rows kFp8SameRows = {nullptr, nullptr, nullptr, nullptr, 1, 0};
 
-__global__ void __launch_bounds__(kFp8QuantThreads) fp8_quantize_kernel(
+constexpr int kFp8QuantWarps = 8;
+constexpr int kFp8QuantCols = 1024;  // per warp
+
+__global__ void __launch_bounds__(32 * kFp8QuantWarps, 8) fp8_quantize_kernel(
     const uint16_t* __restrict__ x, int64_t rows, int cols, int64_t ldx, Fp8Rows to, uint8_t* __restrict__ q,
     float* __restrict__ scale, int64_t scale_ld) {
   pdl_wait();  // the previous kernel of the stream has completed
   pdl_trigger();
-  const int blocks = (cols + kFp8Block - 1) / kFp8Block;
-  const int64_t total = rows * blocks;
-  const int sub = threadIdx.x & 15;
-  const int64_t step = (int64_t)gridDim.x * (kFp8QuantThreads / 16);
-  // every lane of a warp makes the same number of turns (the shuffles below)
-  const int64_t first = (int64_t)blockIdx.x * (kFp8QuantThreads / 16) + (threadIdx.x >> 4);
-  const int64_t warp_first = (int64_t)blockIdx.x * (kFp8QuantThreads / 16) + (threadIdx.x >> 5) * 2;
-  for (int64_t i = first, w = warp_first; w < total; i += step, w += step) {
-    const bool live = i < total;
-    const int64_t row = live ? i / blocks : 0;
-    const int b = live ? (int)(i - row * blocks) : 0;
-    const int col = b * kFp8Block + sub * 8;
-    uint4 v = make_uint4(0u, 0u, 0u, 0u);
-    if (live && col < cols) v = ldg_stream(reinterpret_cast<const uint4*>(x + row * ldx + col));
-    const float2 f[4] = {unpack_bf16x2(v.x), unpack_bf16x2(v.y), unpack_bf16x2(v.z), unpack_bf16x2(v.w)};
+  const int lane = threadIdx.x & 31;
+  const int64_t row = (int64_t)blockIdx.x * kFp8QuantWarps + (threadIdx.x >> 5);
+  if (row >= rows) return;
+  const int col0 = blockIdx.y * kFp8QuantCols + lane * 8;
+  uint4 v[4];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    v[u] = make_uint4(0u, 0u, 0u, 0u);
+    if (col0 + 256 * u < cols) v[u] = ldg_stream(reinterpret_cast<const uint4*>(x + row * ldx + col0 + 256 * u));
+  }
+  int64_t dest = row;
+  if (to.top_idx != nullptr && lane < to.top_k) {
+    const int64_t p = row * to.top_k + lane;
+    const int e = checked_expert(to.top_idx[p], to.experts);
+    dest = (int64_t)to.pcsr[e] + to.inverse[p] - to.csr[e];
+  }
+  uint2 codes[4];
+  float s[4];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const float2 f[4] = {unpack_bf16x2(v[u].x), unpack_bf16x2(v[u].y), unpack_bf16x2(v[u].z), unpack_bf16x2(v[u].w)};
     float a = kFp8MinAmax;
 #pragma unroll
     for (int j = 0; j < 4; ++j) a = fmaxf(a, fmaxf(fabsf(f[j].x), fabsf(f[j].y)));
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
     const float r = div_rn(kE4m3Max, a);
-    const uint2 codes = make_uint2(cvt_e4m3x4(mul_rn(f[0].x, r), mul_rn(f[0].y, r), mul_rn(f[1].x, r), mul_rn(f[1].y, r)),
-                                   cvt_e4m3x4(mul_rn(f[2].x, r), mul_rn(f[2].y, r), mul_rn(f[3].x, r), mul_rn(f[3].y, r)));
-    if (!live) continue;
-    const float s = div_rn(a, kE4m3Max);
-    if (to.top_idx == nullptr) {
-      if (col < cols) *reinterpret_cast<uint2*>(q + row * cols + col) = codes;
-      if (sub == 0) scale[(int64_t)b * scale_ld + row] = s;
-    } else {
-      for (int j = 0; j < to.top_k; ++j) {
-        const int64_t p = row * to.top_k + j;
-        const int e = checked_expert(to.top_idx[p], to.experts);
-        const int64_t dest = (int64_t)to.pcsr[e] + to.inverse[p] - to.csr[e];
-        if (col < cols) *reinterpret_cast<uint2*>(q + dest * cols + col) = codes;
-        if (sub == 0) scale[(int64_t)b * scale_ld + dest] = s;
+    s[u] = div_rn(a, kE4m3Max);
+    codes[u] = make_uint2(cvt_e4m3x4(mul_rn(f[0].x, r), mul_rn(f[0].y, r), mul_rn(f[1].x, r), mul_rn(f[1].y, r)),
+                          cvt_e4m3x4(mul_rn(f[2].x, r), mul_rn(f[2].y, r), mul_rn(f[3].x, r), mul_rn(f[3].y, r)));
+  }
+  for (int j = 0; j < to.top_k; ++j) {
+    const int64_t d = (int64_t)__shfl_sync(0xffffffffu, (unsigned long long)dest, j);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int col = col0 + 256 * u;
+      if (col < cols) {
+        *reinterpret_cast<uint2*>(q + d * cols + col) = codes[u];
+        if ((lane & 15) == 0) scale[(int64_t)(col / kFp8Block) * scale_ld + d] = s[u];
       }
     }
   }
@@ -143,16 +150,24 @@ __global__ void __launch_bounds__(256) fp8_pack_kernel(const uint16_t* __restric
 // the weight rows, so a k-block brings 32 KB per SM instead of 48).
 //
 // warp 0      TMA producer: per k-block of 128 columns the A rows and the
-//             weight rows in boxes of 64 rows (128-byte swizzle)
-// warp 1      MMA issuer (leader CTA): per k-block two MMA groups of 128
-//             columns ("halves"), each into one of its two tensor-memory
-//             buffers: 4 x 128 columns are all 512
-// warps 4..11 epilogue: half h = (warp - 4) / 4 belongs to four warps, one per
-//             lane quadrant. Per k-block a thread reads the 128 columns of its
-//             row in four loads, the next in flight while it adds the last,
-//             times sx * sw, to 128 registers. A buffer is free again as soon
-//             as it is read, 3 MMA groups (768 clocks) before the issuer needs
-//             it.
+//             weight rows (128-byte swizzle)
+// warp 1      MMA issuer (leader CTA): per k-block one group of 4 MMAs into one
+//             of the two tensor-memory buffers of 256 columns
+// warp 2      relay: waits for a group's commit and meets the epilogue warps at
+//             a named barrier
+// warp 3      relay of the pair's second CTA: tells the leader that its epilogue
+//             has read a buffer
+// warps 4..11 epilogue: two warps per lane quadrant, 128 of the 256 columns
+//             each. Per k-block a thread reads its row's 128 columns in eight
+//             loads, the next in flight while it adds the last, times sx * sw,
+//             to 128 registers, and gives the buffer back as soon as it is read.
+//
+// A buffer's round trip (products 512 clocks, commit, sums 260, release, next
+// issue) decides the rate, and what the warps wait on decides the round trip:
+// with one CTA and operands at rest a k-block takes 620 clocks where the
+// epilogue and the issuer meet at named barriers, 805 where every epilogue warp
+// waits on the commit's mbarrier and arrives on another, 680 and 900 with 16
+// epilogue warps of 64 columns.
 //
 // Bound: 128 x 256 x 128 products are 512 clocks of one SM's tensor core; the
 // FMAs of the 128 x 256 block sums are 256 clocks of its fp32 lanes.
@@ -162,7 +177,7 @@ enum Fp8Mode : int { FP8_PLAIN = 0, FP8_SWIGLU = 1 };
 struct Fp8GemmParams {
   CUtensorMap tmap_a;    // activation codes [rows, K], boxes of 128 rows
   CUtensorMap tmap_b;    // weight codes [E * N, K], boxes of 128 rows
-  CUtensorMap tmap_out;  // bf16 output [rows, N], boxes of 32 rows x 64 columns (FP8_PLAIN, N % 8 == 0)
+  CUtensorMap tmap_out;  // bf16 output [rows, N], boxes of 32 rows x 64 columns (tma_out)
   const float* xs;       // activation scales, [K blocks][xs_ld]
   int64_t xs_ld;
   const float* ws;       // weight scales [E][N blocks][K blocks]
@@ -173,11 +188,16 @@ struct Fp8GemmParams {
   int32_t K;
   int32_t experts;
   uint16_t* out;         // FP8_PLAIN: [rows, N]
-  int32_t tma_out;
+  int32_t tma_out;       // N % 8 == 0 and a 16-byte aligned output
   uint8_t* hq;           // FP8_SWIGLU: hidden codes [rows, N / 2]
   float* hs;             // FP8_SWIGLU: hidden scales, [N / 256][hs_ld]
   int64_t hs_ld;
 };
+
+// Named barriers (the last two kinds one per tensor-memory buffer).
+constexpr uint32_t kFp8BarMax = 1;   // SwiGLU row maxima: the epilogue warps
+constexpr uint32_t kFp8BarSums = 2;  // a buffer holds its block sums: relay -> epilogue
+constexpr uint32_t kFp8BarGo = 4;    // a buffer is read and its next operands are there: epilogue, relay -> issuer
 
 template <int CTAS>
 struct Fp8Shape {
@@ -185,11 +205,11 @@ struct Fp8Shape {
   static constexpr int B_BYTES = 256 / CTAS * 128;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
   static constexpr int STAGES = CTAS == 2 ? 6 : 4;
-  static constexpr int EPI_WARPS = 8;
   static constexpr int OUT_BOX = 4096;  // 32 rows x 64 bf16 per epilogue warp
-  // Registers: 12 warps launch with 168 each (64512 in all); the four warps
-  // of the producer and the issuer give some back, and the epilogue's 128
-  // sums and two 32-column loads in flight fit without spilling.
+  static constexpr int EPI_WARPS = 8;
+  // Registers: 12 warps launch with 168 each (64512 in all); the first four
+  // give some back, and the epilogue's 128 sums and two 16-column loads in
+  // flight fit without spilling.
   static constexpr int EPI_WARP0 = 4;
   static constexpr int THREADS = 32 * (EPI_WARP0 + EPI_WARPS);
   static constexpr int LAUNCH_REGS = 168, FRONT_REGS = 40, EPI_REGS = 232;
@@ -232,29 +252,32 @@ __device__ __forceinline__ void fp8_commit(uint64_t* bar) {
   else tc_commit_pair(bar, 0x3);
 }
 
-// acc[0..7] += f * (the 16 columns in r), one FMA each. The statements are
-// volatile, so they stay behind the wait for the loads of r.
-__device__ __forceinline__ void fp8_add_block(uint64_t* acc, const uint32_t (&r)[16], float f) {
+// acc[0..15] += f * (the 16 columns in r). The statements are volatile, so they
+// stay behind the wait for the loads of r.
+__device__ __forceinline__ void fp8_add_block(float* acc, const uint32_t (&r)[16], float f) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
-    asm volatile(
-        "{\n\t.reg .b64 d, s;\n\tmov.b64 d, {%1, %2};\n\tmov.b64 s, {%3, %3};\n\t"
-        "fma.rn.f32x2 %0, d, s, %0;\n\t}"
-        : "+l"(acc[j])
-        : "r"(r[2 * j]), "r"(r[2 * j + 1]), "f"(f));
-}
-__device__ __forceinline__ float2 unpack_f32x2(uint64_t v) {
-  return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
+  for (int j = 0; j < 16; ++j)
+    asm volatile("fma.rn.f32 %0, %1, %2, %0;" : "+f"(acc[j]) : "f"(__uint_as_float(r[j])), "f"(f));
 }
 
-// mbar_wait (common.cuh) that looks at the clock only every 64 tries: a wait
-// per k-block and role is on the path of every MMA here, and the first read of
-// %globaltimer alone costs about as much as a k-block's products.
+// mbar_wait (common.cuh) for waits on the path of every MMA: each try may
+// suspend the warp for up to 100 us of its own (polling warps take issue slots
+// and shared-memory cycles from the others), and the clock is read every 64
+// tries.
 __device__ __forceinline__ bool fp8_wait(uint64_t* bar, uint32_t parity, unsigned int code,
                                          uint64_t limit_ns = 2000000000ull, bool stop_on_error = true) {
+  const uint32_t addr = smem_u32(bar);
   uint64_t start = 0;
   for (uint32_t i = 1;; ++i) {
-    if (mbar_try_wait(bar, parity)) return true;
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(addr), "r"(parity), "r"(100000u)
+        : "memory");
+    if (done) return true;
     if ((i & 63u) == 0u) {
       if (stop_on_error && error_raised()) return false;
       const uint64_t now = globaltimer_ns();
@@ -281,21 +304,26 @@ __device__ __forceinline__ void regs_down() {
 template <int CTAS>
 __device__ __forceinline__ TileEntry fp8_tile(const Fp8GemmParams& p, int m) {
   if (p.tiles != nullptr) {
-    TileEntry t = p.tiles[m];
-    if (CTAS == 1) t.pad = kTileRows;  // rows that may be stored
-    return t;
+    return p.tiles[m];
   }
   TileEntry t;
   t.expert = 0;
   t.row0 = m * CTAS * kTileRows;
   t.valid = (int32_t)min((int64_t)CTAS * kTileRows, p.rows - t.row0);
-  t.pad = t.valid;
+  t.pad = 0;
   return t;
 }
 
-// g / (1 + exp(-g)) * u
-__device__ __forceinline__ float swiglu_f32(float g, float u) {
-  return __fdividef(1.0f, 1.0f + __expf(-g)) * g * u;
+// g / (1 + exp(-g)) * u for two columns, in place of the gates. One reciprocal
+// serves both: 1 / (d0 d1) times the other denominator. exp(-g) is held below
+// e^40, so that the product stays finite; a gate below -40 then gives up to
+// 40 e^-40 = 2e-16 instead of less, which no E4M3 block can tell from 0 beside
+// values above 1e-12.
+__device__ __forceinline__ void swiglu_pair_f32(float& g0, float& g1, float u0, float u1) {
+  const float d0 = 1.0f + __expf(fminf(-g0, 40.0f)), d1 = 1.0f + __expf(fminf(-g1, 40.0f));
+  const float r = __fdividef(1.0f, d0 * d1);
+  g0 *= r * d1 * u0;
+  g1 *= r * d0 * u1;
 }
 
 // Tensor-memory column of a thread's chunk c of 16 columns, from its first.
@@ -313,12 +341,12 @@ __device__ __forceinline__ void fp8_gemm_body(const Fp8GemmParams& p) {
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sA = smem;
   uint8_t* sB = sA + S::STAGES * S::A_BYTES;
-  uint8_t* sOut = sB + S::STAGES * S::B_BYTES;  // output boxes; FP8_SWIGLU: row maxima [2 units][2 halves][128]
+  uint8_t* sOut = sB + S::STAGES * S::B_BYTES;
+  float* s_max = reinterpret_cast<float*>(sOut);  // FP8_SWIGLU: row maxima [unit parity][half][row]
   uint64_t* full = reinterpret_cast<uint64_t*>(sOut + S::EPI_WARPS * S::OUT_BOX);
-  uint64_t* empty = full + S::STAGES;
-  uint64_t* acc_full = empty + S::STAGES;  // per buffer
-  uint64_t* acc_empty = acc_full + 2;      // per buffer, the leader's
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  uint64_t* done = full + S::STAGES;       // products of a stage complete: its sums are there, its memory is free
+  uint64_t* peer_free = done + S::STAGES;  // per buffer, the leader's: its peer has read it
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(peer_free + 2);
 
   const int warp = threadIdx.x >> 5;
   const uint32_t lane = threadIdx.x & 31;
@@ -327,12 +355,9 @@ __device__ __forceinline__ void fp8_gemm_body(const Fp8GemmParams& p) {
   if (threadIdx.x == 0) {
     for (int s = 0; s < S::STAGES; ++s) {
       mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
+      mbar_init(&done[s], 1);
     }
-    for (int b = 0; b < 2; ++b) {
-      mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], S::EPI_WARPS * CTAS);
-    }
+    for (int b = 0; b < 2; ++b) mbar_init(&peer_free[b], S::EPI_WARPS);
     fence_barrier_init();
   }
   if (warp == 0 && lane == 0) {
@@ -362,37 +387,40 @@ __device__ __forceinline__ void fp8_gemm_body(const Fp8GemmParams& p) {
   const int total = num_m * n_tiles;
   const int k_blocks = (p.K + kFp8Block - 1) / kFp8Block;
   const int first = blockIdx.x / CTAS, step = gridDim.x / CTAS;
+  // k-blocks of this CTA: every role below takes exactly this many turns, on
+  // every path, so that the named barriers stay matched (the issuer commits
+  // each turn, so the waits for its commits end too)
+  const int turns = first < total ? ((total - 1 - first) / step + 1) * k_blocks : 0;
 
   if (warp < S::EPI_WARP0) {
     regs_down<S::FRONT_REGS>();
-    if (warp == 0 && lane == 0) {
+    if (warp == 0) {
       // ---------------- TMA producer (every CTA) ----------------
+      // one lane per copy: A, the first 128 weight rows, the next 128 (CTAS = 1)
       const uint32_t full_leader = CTAS == 1 ? 0u : mapa_shared(smem_u32(full), 0);
+      constexpr uint32_t kCopies = CTAS == 1 ? 3 : 2;
+      const CUtensorMap* map = lane == 0 ? &p.tmap_a : &p.tmap_b;
+      uint8_t* const dst0 = lane == 0 ? sA : sB + (lane == 2 ? 16384 : 0);
+      const uint32_t dst_step = lane == 0 ? S::A_BYTES : S::B_BYTES;
       uint32_t stage = 0, phase = 0;
       bool ok = true;
       for (int u = first; u < total && ok; u += step) {
         const int m = u / n_tiles, n = u - m * n_tiles;
         const TileEntry t = fp8_tile<CTAS>(p, m);
-        const int a_row = t.row0 + 128 * (int)rank;
-        // the weight rows of columns 0..127 (leader) and 128..255 (its peer)
-        const int b_row = t.expert * p.N + (MODE == FP8_SWIGLU ? n * 128 : n * 256);
-        const int b_up = MODE == FP8_SWIGLU ? F : 128;
+        // weight rows of columns 0..127 and 128..255 (of the leader and its peer)
+        const int part = CTAS == 1 ? (lane == 2 ? 1 : 0) : (int)rank;
+        const int row = lane == 0 ? t.row0 + 128 * (int)rank
+                                  : t.expert * p.N + (MODE == FP8_SWIGLU ? n * 128 + part * F : n * 256 + part * 128);
         for (int kb = 0; kb < k_blocks; ++kb) {
-          if (!fp8_wait(&empty[stage], phase ^ 1u, kErrTimeoutProducer)) {
-            ok = false;
-            break;
-          }
-          if (rank == 0) mbar_arrive_expect_tx(&full[stage], CTAS * S::STAGE_BYTES);
-          uint8_t* a = sA + stage * S::A_BYTES;
-          uint8_t* b = sB + stage * S::B_BYTES;
-          if constexpr (CTAS == 1) {
-            tma_load_2d(a, &p.tmap_a, &full[stage], kb * 128, a_row);
-            tma_load_2d(b, &p.tmap_b, &full[stage], kb * 128, b_row);
-            tma_load_2d(b + 16384, &p.tmap_b, &full[stage], kb * 128, b_row + b_up);
-          } else {
-            const uint32_t fb = full_leader + stage * 8;
-            tma_load_2d_pair(a, &p.tmap_a, fb, kb * 128, a_row);
-            tma_load_2d_pair(b, &p.tmap_b, fb, kb * 128, b_row + (int)rank * b_up);
+          ok = fp8_wait(&done[stage], phase ^ 1u, kErrTimeoutProducer);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          if (rank == 0 && lane == 0) mbar_arrive_expect_tx(&full[stage], CTAS * S::STAGE_BYTES);
+          __syncwarp();
+          if (lane < kCopies) {
+            uint8_t* dst = dst0 + stage * dst_step;
+            if constexpr (CTAS == 1) tma_load_2d(dst, map, &full[stage], kb * 128, row);
+            else tma_load_2d_pair(dst, map, full_leader + stage * 8, kb * 128, row);
           }
           if (++stage == S::STAGES) {
             stage = 0;
@@ -400,181 +428,208 @@ __device__ __forceinline__ void fp8_gemm_body(const Fp8GemmParams& p) {
           }
         }
       }
-      // after an error the copies in flight still land before the CTA ends
-      if (!ok && rank == 0)
-        for (uint32_t s = 0; s < S::STAGES; ++s)
-          fp8_wait(&full[s], s < stage ? phase : phase ^ 1u, kErrTimeoutProducer, 50000000ull, false);
-    } else if (warp == 1 && lane == 0 && rank == 0) {
+    } else if (warp == 1 && rank == 0) {
       // ---------------- MMA issuer (leader) ----------------
       constexpr uint32_t idesc = idesc_e4m3(128 * CTAS, 256);
       const uint64_t a_desc = smem_desc(smem_u32(sA), 16, 1024, kLayoutSwizzle128B);
       const uint32_t desc_hi = (uint32_t)(a_desc >> 32), a_lo = (uint32_t)a_desc;
       const uint32_t b_lo = (uint32_t)smem_desc(smem_u32(sB), 16, 1024, kLayoutSwizzle128B);
-      uint32_t stage = 0, phase = 0, cnt = 0;
-      bool ok = true;
-      for (int u = first; u < total && ok; u += step) {
-        for (int kb = 0; kb < k_blocks && ok; ++kb, ++cnt) {
-          const uint32_t buf = cnt & 1u, buf_phase = (cnt >> 1) & 1u;
-          ok = fp8_wait(&full[stage], phase, kErrTimeoutMma);
-          if (!ok) break;
+      uint32_t stage = 0, buf = 0;
+      for (int i = 0; i < turns; ++i, buf ^= 1u) {
+        named_sync(kFp8BarGo + buf, i < 2 ? 64 : 32 * (S::EPI_WARPS + 2));
+        tc_fence_after();
+        if (lane == 0) {
           const uint32_t a = a_lo + stage * (S::A_BYTES >> 4), b = b_lo + stage * (S::B_BYTES >> 4);
-          ok = fp8_wait(&acc_empty[buf], buf_phase ^ 1u, kErrTimeoutMma);
-          if (!ok) break;
-          tc_fence_after();
           const uint32_t d = tmem + buf * 256;
           tc_mma_e4m3<CTAS, 0>(d, a, b, desc_hi, idesc);
           tc_mma_e4m3<CTAS, 1>(d, a + 2, b + 2, desc_hi, idesc);
           tc_mma_e4m3<CTAS, 1>(d, a + 4, b + 4, desc_hi, idesc);
           tc_mma_e4m3<CTAS, 1>(d, a + 6, b + 6, desc_hi, idesc);
-          fp8_commit<CTAS>(&acc_full[buf]);
-          fp8_commit<CTAS>(&empty[stage]);
-          if (++stage == S::STAGES) {
-            stage = 0;
-            phase ^= 1u;
-          }
+          fp8_commit<CTAS>(&done[stage]);
+        }
+        __syncwarp();
+        if (++stage == S::STAGES) stage = 0;
+      }
+      // the epilogue's releases of the last two buffers
+      for (int i = turns < 2 ? 0 : turns - 2; i < turns; ++i)
+        named_sync(kFp8BarGo + (i & 1), 32 * (S::EPI_WARPS + 2));
+    } else if (warp == 2) {
+      // ---------------- relay: products complete -> epilogue (every CTA) ----------------
+      uint32_t stage = 0, phase = 0;
+      for (int i = 0; i < turns; ++i) {
+        fp8_wait(&done[stage], phase, kErrTimeoutEpilogue, 2000000000ull, false);
+        __syncwarp();
+        named_sync(kFp8BarSums + (i & 1), 32 * (S::EPI_WARPS + 1));
+        if (++stage == S::STAGES) {
+          stage = 0;
+          phase ^= 1u;
         }
       }
+    } else if (warp == 3 && rank == 0) {
+      // ---------------- relay: operands landed, peer's buffer read -> issuer (leader) ----------------
+      // takes part in the go barrier for what would be waits of the issuer
+      uint32_t stage = 0, stage_phase = 0, buf = 0, phase = 0;
+      bool ok = true;
+      for (int i = 0; i < turns; ++i) {
+        ok = ok && fp8_wait(&full[stage], stage_phase, kErrTimeoutMma);
+        if (CTAS == 2 && i >= 2) fp8_wait(&peer_free[buf], phase ^ 1u, kErrTimeoutMma, 2000000000ull, false);
+        __syncwarp();
+        named_sync(kFp8BarGo + buf, i < 2 ? 64 : 32 * (S::EPI_WARPS + 2));
+        if (++stage == S::STAGES) {
+          stage = 0;
+          stage_phase ^= 1u;
+        }
+        phase ^= buf;
+        buf ^= 1u;
+      }
+      for (int i = turns < 2 ? 0 : turns - 2; i < turns; ++i)
+        named_sync(kFp8BarGo + (i & 1), 32 * (S::EPI_WARPS + 2));
     }
   } else {
     regs_up<S::EPI_REGS>();
-    // ---------------- epilogue (warps 4..11, every CTA) ----------------
-    // After a wait that gave up the warps go through the remaining units
-    // without waiting or storing, so that the named barriers stay matched.
+    // ---------------- epilogue (warps 4..19, every CTA) ----------------
     const uint32_t quad = (uint32_t)(warp & 3);
-    const int h = (warp - S::EPI_WARP0) >> 2;
+    const int h = (warp - S::EPI_WARP0) >> 2;  // columns 128 h .. (SwiGLU: gate 64 h .. and up 128 + 64 h ..)
     const int row_in_cta = (int)(quad * 32 + lane);
-    const uint32_t acc_empty_leader = CTAS == 1 ? 0u : mapa_shared(smem_u32(acc_empty), 0);
-    // SwiGLU: 64 gate columns and the up columns 128 further on; else 128 in a row
+    const uint32_t peer_free_leader = CTAS == 1 ? 0u : mapa_shared(smem_u32(peer_free), 0);
     const uint32_t taddr = tmem + ((quad * 32u) << 16) + (MODE == FP8_SWIGLU ? 64u : 128u) * h;
-    uint8_t* box = sOut + (warp - S::EPI_WARP0) * S::OUT_BOX;
     const int n_blocks = (p.N + kFp8Block - 1) / kFp8Block;
-    uint32_t cnt = 0, unit = 0;
-    bool ok = true;
-    for (int u = first; u < total; u += step, ++unit) {
-      const int m = u / n_tiles, n = u - m * n_tiles;
+    // A unit's rows, columns and scale addresses, and the scales of its first
+    // two k-blocks, are fetched while the previous unit is written out.
+    const int row_in_tile = row_in_cta + 128 * (int)rank;
+    const int64_t up = MODE == FP8_SWIGLU ? (int64_t)(F / 128) * k_blocks : 0;
+    int n = 0, valid = 0;
+    int64_t row = 0;
+    const float *xs = nullptr, *ws = nullptr;
+    float x0 = 0.0f, w00 = 0.0f, w01 = 0.0f, x1 = 0.0f, w10 = 0.0f, w11 = 0.0f;
+    auto fetch = [&](int u) {
+      const int m = u / n_tiles;
       const TileEntry t = fp8_tile<CTAS>(p, m);
-      const int row_in_tile = row_in_cta + 128 * (int)rank;
-      const int64_t row = (int64_t)t.row0 + row_in_tile;
-      const float* xs = p.xs + min(row, p.rows - 1);
+      n = u - m * n_tiles;
+      valid = t.valid;
+      row = (int64_t)t.row0 + row_in_tile;
+      xs = p.xs + min(row, p.rows - 1);
       // the weight scales of this thread's columns: one row of blocks, or the
-      // gate's (columns 0..63) and the up's (64..127)
+      // gate's and the up's
       const int nb0 = MODE == FP8_SWIGLU ? n : min(2 * n + h, n_blocks - 1);
-      const int nb1 = MODE == FP8_SWIGLU ? n + F / 128 : nb0;
-      const float* ws0 = p.ws + ((int64_t)t.expert * n_blocks + nb0) * k_blocks;
-      const float* ws1 = p.ws + ((int64_t)t.expert * n_blocks + nb1) * k_blocks;
-      uint64_t acc[64];  // two neighbouring columns each
+      ws = p.ws + ((int64_t)t.expert * n_blocks + nb0) * k_blocks;
+      x0 = __ldg(xs);
+      w00 = __ldg(ws);
+      if (MODE == FP8_SWIGLU) w01 = __ldg(ws + up);
+      if (k_blocks > 1) {
+        x1 = __ldg(xs + p.xs_ld);
+        w10 = __ldg(ws + 1);
+        if (MODE == FP8_SWIGLU) w11 = __ldg(ws + 1 + up);
+      }
+    };
+    uint32_t buf = 0, unit = 0;
+    if (first < total) fetch(first);
+    for (int u = first; u < total; u += step, ++unit) {
+      float acc[128];
 #pragma unroll
-      for (int j = 0; j < 64; ++j) acc[j] = 0;
-      float f0 = __ldg(xs) * __ldg(ws0), f1 = MODE == FP8_SWIGLU ? __ldg(xs) * __ldg(ws1) : f0;
+      for (int j = 0; j < 128; ++j) acc[j] = 0.0f;
       uint32_t ra[16], rb[16];
-      ok = ok && fp8_wait(&acc_full[cnt & 1u], (cnt >> 1) & 1u, kErrTimeoutEpilogue);
-      tc_fence_after();
-      tc_ld_32x32b_x16(taddr + (cnt & 1u) * 256, ra);
-      for (int kb = 0; kb < k_blocks; ++kb, ++cnt) {
-        const uint32_t buf = cnt & 1u, tb = taddr + buf * 256;
-        float sx = 0.0f, w0 = 0.0f, w1 = 0.0f;
-        if (kb + 1 < k_blocks) {
-          sx = __ldg(xs + (int64_t)(kb + 1) * p.xs_ld);
-          w0 = __ldg(ws0 + kb + 1);
-          if (MODE == FP8_SWIGLU) w1 = __ldg(ws1 + kb + 1);
+      for (int kb = 0; kb < k_blocks; ++kb, buf ^= 1u) {
+        const uint32_t tb = taddr + buf * 256;
+        const float f0 = x0 * w00, f1 = MODE == FP8_SWIGLU ? x0 * w01 : f0;
+        x0 = x1;
+        w00 = w10;
+        w01 = w11;
+        if (kb + 2 < k_blocks) {  // two blocks ahead of their use
+          x1 = __ldg(xs + (int64_t)(kb + 2) * p.xs_ld);
+          w10 = __ldg(ws + kb + 2);
+          if (MODE == FP8_SWIGLU) w11 = __ldg(ws + kb + 2 + up);
         }
+        named_sync(kFp8BarSums + buf, 32 * (S::EPI_WARPS + 1));
+        tc_fence_after();
+        tc_ld_32x32b_x16(tb, ra);
 #pragma unroll
         for (int c = 0; c < 8; c += 2) {
-          const float f = c < 4 ? f0 : f1;
           tc_wait_ld();
           tc_ld_32x32b_x16(tb + chunk_col<MODE>(c + 1), rb);
-          fp8_add_block(acc + 8 * c, ra, f);
+          fp8_add_block(acc + 16 * c, ra, c < 4 ? f0 : f1);
           if (c == 6) break;
           tc_wait_ld();
           tc_ld_32x32b_x16(tb + chunk_col<MODE>(c + 2), ra);
-          fp8_add_block(acc + 8 * (c + 1), rb, f);
+          fp8_add_block(acc + 16 * (c + 1), rb, c < 4 ? f0 : f1);
         }
         tc_wait_ld();
         tc_fence_before();
-        __syncwarp();
-        if (lane == 0) {
-          if (CTAS == 1 || rank == 0) mbar_arrive(&acc_empty[buf]);
-          else mbar_arrive_cluster(acc_empty_leader + buf * 8);
+        if (CTAS == 1 || rank == 0) {
+          named_arrive(kFp8BarGo + buf, 32 * (S::EPI_WARPS + 2));
+        } else {
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(peer_free_leader + buf * 8);
         }
-        if (kb + 1 < k_blocks) {
-          const uint32_t next = cnt + 1;
-          ok = ok && fp8_wait(&acc_full[next & 1u], (next >> 1) & 1u, kErrTimeoutEpilogue);
-          tc_fence_after();
-          tc_ld_32x32b_x16(taddr + (next & 1u) * 256, ra);
-        }
-        fp8_add_block(acc + 56, rb, f1);
-        f0 = sx * w0;
-        f1 = MODE == FP8_SWIGLU ? sx * w1 : f0;
+        fp8_add_block(acc + 112, rb, f1);
       }
+      const int n_out = n;
+      const int64_t row_out = row;
+      const bool store = row_in_tile < valid;
+      if (u + step < total) fetch(u + step);
       if constexpr (MODE == FP8_SWIGLU) {
-        // 64 hidden columns 128 n + 64 h ..; the other half's warps hold the
+        // 64 hidden columns 128 n_out + 64 h ..; the other half's warps hold the
         // rest of the row's block, so the row maxima meet in shared memory
         float a = kFp8MinAmax;
-        float2 hid[32];
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          const float2 g = unpack_f32x2(acc[j]), v = unpack_f32x2(acc[32 + j]);
-          hid[j] = make_float2(swiglu_f32(g.x, v.x), swiglu_f32(g.y, v.y));
-          a = fmaxf(a, fmaxf(fabsf(hid[j].x), fabsf(hid[j].y)));
+        for (int j = 0; j < 64; j += 2) {
+          swiglu_pair_f32(acc[j], acc[j + 1], acc[64 + j], acc[65 + j]);
+          a = fmaxf(a, fmaxf(fabsf(acc[j]), fabsf(acc[j + 1])));
         }
-        float* s_max = reinterpret_cast<float*>(sOut) + (unit & 1u) * 256;
-        s_max[h * 128 + row_in_cta] = a;
-        named_sync(1, 32 * S::EPI_WARPS);
-        a = fmaxf(a, s_max[(h ^ 1) * 128 + row_in_cta]);
-        if (ok && row_in_tile < t.valid) {
+        float* mx = s_max + (unit & 1u) * 256 + row_in_cta;
+        mx[h * 128] = a;
+        named_sync(kFp8BarMax, 32 * S::EPI_WARPS);
+        a = fmaxf(a, mx[(h ^ 1) * 128]);
+        if (store) {
           const float r = div_rn(kE4m3Max, a);
-          uint4* dst = reinterpret_cast<uint4*>(p.hq + row * F + n * 128 + 64 * h);
+          uint8_t* dst = p.hq + row_out * F + n_out * 128 + 64 * h;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            uint32_t c[4];
+          for (int j = 0; j < 2; ++j) {
+            uint32_t c[8];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float2 v0 = hid[8 * j + 2 * i], v1 = hid[8 * j + 2 * i + 1];
-              c[i] = cvt_e4m3x4(mul_rn(v0.x, r), mul_rn(v0.y, r), mul_rn(v1.x, r), mul_rn(v1.y, r));
+            for (int i = 0; i < 8; ++i) {
+              const float* v = acc + 32 * j + 4 * i;
+              c[i] = cvt_e4m3x4(mul_rn(v[0], r), mul_rn(v[1], r), mul_rn(v[2], r), mul_rn(v[3], r));
             }
-            dst[j] = make_uint4(c[0], c[1], c[2], c[3]);
+            st_global_v8(reinterpret_cast<uint16_t*>(dst + 32 * j), make_uint4(c[0], c[1], c[2], c[3]),
+                         make_uint4(c[4], c[5], c[6], c[7]));
           }
-          if (h == 0) p.hs[(int64_t)n * p.hs_ld + row] = div_rn(a, kE4m3Max);
+          if (h == 0) p.hs[(int64_t)n_out * p.hs_ld + row_out] = div_rn(a, kE4m3Max);
         }
       } else {
-        const int col0 = n * 256 + 128 * h;
+        const int col0 = n_out * 256 + 128 * h;
         if (p.tma_out) {
-          // two boxes of 32 rows x 64 columns in the TMA 128-byte swizzle; a
-          // table's tile is stored whole (its padding rows are scratch)
-          const int live = t.pad - 128 * (int)rank - 32 * (int)quad;
+          // two boxes of 32 rows x 64 columns in the TMA 128-byte swizzle; of a
+          // table's tile the padding rows are written too (scratch), never
+          // rows of the next tile
+          uint8_t* box = sOut + (warp - S::EPI_WARP0) * S::OUT_BOX;
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             if (lane == 0) bulk_wait_group_read0();
             __syncwarp();
 #pragma unroll
             for (int c = 0; c < 8; ++c) {
-              uint32_t w[4];
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const float2 v = unpack_f32x2(acc[i * 32 + c * 4 + j]);
-                w[j] = cvt_bf16x2(v.x, v.y);
-              }
+              const float* v = acc + 64 * i + 8 * c;
               *reinterpret_cast<uint4*>(box + lane * 128 + ((c ^ (lane & 7)) << 4)) =
-                  make_uint4(w[0], w[1], w[2], w[3]);
+                  make_uint4(cvt_bf16x2(v[0], v[1]), cvt_bf16x2(v[2], v[3]), cvt_bf16x2(v[4], v[5]),
+                             cvt_bf16x2(v[6], v[7]));
             }
             fence_proxy_async_shared();
             __syncwarp();
-            if (lane == 0 && ok && live > 0 && col0 + 64 * i < p.N) {
-              tma_store_2d(&p.tmap_out, box, col0 + 64 * i, t.row0 + 128 * (int)rank + 32 * (int)quad);
+            if (lane == 0 && store && col0 + 64 * i < p.N) {  // row 0 of the box has a routed row
+              tma_store_2d(&p.tmap_out, box, col0 + 64 * i, (int32_t)row_out);
               bulk_commit_group();
             }
           }
-        } else if (ok && row_in_tile < t.valid) {
+        } else if (store) {
           // rows of N bf16 that are not multiples of 16 bytes
-          uint16_t* dst = p.out + row * p.N + col0;
+          uint16_t* dst = p.out + row_out * p.N + col0;
 #pragma unroll
-          for (int j = 0; j < 64; ++j) {
-            const float2 v = unpack_f32x2(acc[j]);
-            if (col0 + 2 * j < p.N) dst[2 * j] = f32_to_bf16(v.x);
-            if (col0 + 2 * j + 1 < p.N) dst[2 * j + 1] = f32_to_bf16(v.y);
-          }
+          for (int j = 0; j < 128; ++j)
+            if (col0 + j < p.N) dst[j] = f32_to_bf16(acc[j]);
         }
       }
+      __syncwarp();
     }
     if (MODE == FP8_PLAIN && lane == 0) bulk_wait_group0();
   }
@@ -604,13 +659,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Fp8Shape<2>::THREADS
 // ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
+// Rows of `cols` elements in boxes of 128 bytes x box_rows, 128-byte swizzle.
 static int fp8_map(CUtensorMap* map, CUtensorMapDataType type, int elem, const void* base, int64_t rows, int64_t cols,
-                   int box_cols, int box_rows) {
+                   int box_rows) {
   EncodeTiledFn fn = encode_fn();
   if (fn == nullptr) return set_error(PRAXIS_B200_ECUDA, "cuTensorMapEncodeTiled is unavailable");
   cuuint64_t gdim[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
   cuuint64_t gstride[1] = {(cuuint64_t)cols * elem};
-  cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
+  cuuint32_t box[2] = {(cuuint32_t)(128 / elem), (cuuint32_t)box_rows};
   cuuint32_t estride[2] = {1u, 1u};
   CUresult r = fn(map, type, 2, const_cast<void*>(base), gdim, gstride, box, estride, CU_TENSOR_MAP_INTERLEAVE_NONE,
                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -668,12 +724,10 @@ static int fp8_launch(const Fp8GemmParams& p, int64_t units, cudaStream_t stream
 int run_fp8_quantize(const uint16_t* x, int64_t rows, int cols, int64_t ldx, const Fp8Rows& to, uint8_t* q,
                      float* scale, int64_t scale_ld, cudaStream_t stream) {
   if (rows == 0) return PRAXIS_B200_OK;
-  const int64_t blocks = rows * ((cols + kFp8Block - 1) / kFp8Block);
-  int64_t grid = (blocks + kFp8QuantThreads / 16 - 1) / (kFp8QuantThreads / 16);
-  const int64_t most = (int64_t)sm_count() * 8;
-  if (grid > most) grid = most;
-  launch_pdl(fp8_quantize_kernel, dim3((unsigned)grid), dim3(kFp8QuantThreads), 0, stream, x, rows, cols, ldx, to, q,
-             scale, scale_ld);
+  const dim3 grid((unsigned)((rows + kFp8QuantWarps - 1) / kFp8QuantWarps),
+                  (unsigned)((cols + kFp8QuantCols - 1) / kFp8QuantCols));
+  launch_pdl(fp8_quantize_kernel, grid, dim3(32 * kFp8QuantWarps), 0, stream, x, rows, cols, ldx, to, q, scale,
+             scale_ld);
   return check_launch("fp8_quantize");
 }
 
@@ -711,13 +765,13 @@ int run_fp8_gemm(const Fp8Gemm& g, cudaStream_t stream) {
   if (g.rows == 0) return PRAXIS_B200_OK;
   Fp8GemmParams p;
   memset(&p, 0, sizeof(p));
-  int rc = fp8_map(&p.tmap_a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, g.q, g.rows, g.k, 128, 128);
+  int rc = fp8_map(&p.tmap_a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, g.q, g.rows, g.k, 128);
   if (rc) return rc;
-  rc = fp8_map(&p.tmap_b, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, g.wq, (int64_t)g.experts * g.n, g.k, 128, 128);
+  rc = fp8_map(&p.tmap_b, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, g.wq, (int64_t)g.experts * g.n, g.k, 128);
   if (rc) return rc;
   const bool swiglu = g.out == nullptr;
   if (!swiglu && g.n % 8 == 0 && ((uintptr_t)g.out & 15) == 0) {
-    rc = fp8_map(&p.tmap_out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, g.out, g.rows, g.n, 64, 32);
+    rc = fp8_map(&p.tmap_out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, g.out, g.rows, g.n, 32);
     if (rc) return rc;
     p.tma_out = 1;
   }

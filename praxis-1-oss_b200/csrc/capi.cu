@@ -229,6 +229,7 @@ static Fp8LinearLayout fp8_linear_layout(int64_t rows, int64_t k) {
 
 // The feed-forward: `rows` are the tokens (dense) or the padded routed rows.
 struct Fp8FfnLayout {
+  size_t stream_hidden, stream_y, stream_inverse, stream_top, stream_gate, stream_csr, stream_pcsr;  // streaming path
   size_t dispatch, inverse, csr, pcsr, offsets, tiles, num_tiles, aq, as, hq, hs, rows, total;
   int64_t rp, scale_ld;
   int max_tiles;
@@ -260,6 +261,17 @@ static Fp8FfnLayout fp8_ffn_layout(int64_t tokens, int top_k, int experts, int d
   L.hs = take((size_t)(hidden / 128) * L.scale_ld * 4);
   L.rows = take(routed ? (size_t)L.rp * dim * 2 : 0);
   L.total = off;
+  // The streaming path uses the same bytes: its fp32 hidden rows, and for a
+  // fused tail its output and a dispatch of the tokens to themselves.
+  off = 0;
+  L.stream_hidden = take((size_t)tokens * (routed ? top_k : 1) * hidden * 4);
+  L.stream_y = take((size_t)tokens * dim * 2);
+  L.stream_inverse = take((size_t)tokens * 8);
+  L.stream_top = take((size_t)tokens * 8);
+  L.stream_gate = take((size_t)tokens * 2);
+  L.stream_csr = take(8);
+  L.stream_pcsr = take(8);
+  if (fp8_streams(tokens, top_k, experts) && off > L.total) L.total = off;
   return L;
 }
 
@@ -752,6 +764,19 @@ int praxis_b200_fp8_linear(const void* x, int64_t rows, int32_t k, int64_t ldx, 
   if (workspace_size < L.total)
     return set_error(PRAXIS_B200_EINVAL, "fp8_linear: workspace %zu < %zu bytes", workspace_size, L.total);
   cudaStream_t s = PRAXIS_STREAM(stream);
+  if (fp8_streams(rows, 0, 1)) {
+    Fp8StreamParams p = {};
+    p.x = x;
+    p.ldx = ldx;
+    p.wq = static_cast<const uint8_t*>(w_q);
+    p.ws = w_scale;
+    p.rows = (int32_t)rows;
+    p.N = n;
+    p.K = k;
+    p.experts = 1;
+    p.out = static_cast<uint16_t*>(out);
+    return run_fp8_stream_linear(p, s);
+  }
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   float* scale = reinterpret_cast<float*>(ws + L.scale);
   rc = run_fp8_quantize(static_cast<const uint16_t*>(x), rows, k, ldx, kFp8SameRows, ws + L.q, scale, L.scale_ld, s);
@@ -803,6 +828,35 @@ int praxis_b200_fp8_ffn(const praxis_b200_fp8_ffn_args* a) {
     return set_error(PRAXIS_B200_EINVAL, "fp8_ffn: workspace %zu < %zu bytes", a->workspace_size, L.total);
   cudaStream_t s = PRAXIS_STREAM(a->stream);
   uint8_t* ws = static_cast<uint8_t*>(a->workspace);
+  if (fp8_streams(a->tokens, top_k, a->experts)) {
+    Fp8StreamParams p = {};
+    p.x = a->x;
+    p.ldx = a->dim;
+    p.wq = static_cast<const uint8_t*>(a->gate_up_q);
+    p.ws = a->gate_up_scale;
+    p.rows = (int32_t)a->tokens;
+    p.N = 2 * a->hidden;
+    p.K = a->dim;
+    p.experts = a->experts;
+    p.top_k = top_k;
+    p.top_idx = a->top_idx;
+    p.gate = static_cast<const uint16_t*>(a->gate);
+    p.scaling = a->scaling;
+    p.shared = static_cast<const uint16_t*>(a->shared);
+    p.hidden = reinterpret_cast<float*>(ws + L.stream_hidden);
+    p.out = a->tail ? reinterpret_cast<uint16_t*>(ws + L.stream_y) : static_cast<uint16_t*>(a->out);
+    rc = run_fp8_stream_ffn(p, static_cast<const uint8_t*>(a->down_q), a->down_scale, a->dim, a->hidden, s);
+    if (rc || !a->tail) return rc;
+    int64_t* inverse = reinterpret_cast<int64_t*>(ws + L.stream_inverse);
+    int64_t* top_idx = reinterpret_cast<int64_t*>(ws + L.stream_top);
+    uint16_t* gate = reinterpret_cast<uint16_t*>(ws + L.stream_gate);
+    int32_t* csr = reinterpret_cast<int32_t*>(ws + L.stream_csr);
+    int32_t* pcsr = reinterpret_cast<int32_t*>(ws + L.stream_pcsr);
+    rc = run_fp8_identity((int)a->tokens, inverse, top_idx, gate, csr, pcsr, s);
+    if (rc) return rc;
+    return run_combine_tail(p.out, a->dim, inverse, top_idx, gate, csr, pcsr, nullptr, nullptr, nullptr, 1, 1.0f,
+                            nullptr, tail_args(*a->tail), a->tokens, 1, 1, s);
+  }
   int64_t* inverse = reinterpret_cast<int64_t*>(ws + L.inverse);
   int32_t* csr = reinterpret_cast<int32_t*>(ws + L.csr);
   int32_t* pcsr = reinterpret_cast<int32_t*>(ws + L.pcsr);

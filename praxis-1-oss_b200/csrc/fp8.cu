@@ -15,6 +15,8 @@
 // d_b leaves tensor memory once and is added into registers with one FMA.
 #include <cuda.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "kernels.h"
 
@@ -55,7 +57,7 @@ constexpr Fp8Rows kFp8SameRows = {nullptr, nullptr, nullptr, nullptr, 1, 0};
 constexpr int kFp8QuantWarps = 8;
 constexpr int kFp8QuantCols = 1024;  // per warp
 
-__global__ void __launch_bounds__(32 * kFp8QuantWarps, 8) fp8_quantize_kernel(
+__global__ void __launch_bounds__(32 * kFp8QuantWarps, 6) fp8_quantize_kernel(
     const uint16_t* __restrict__ x, int64_t rows, int cols, int64_t ldx, Fp8Rows to, uint8_t* __restrict__ q,
     float* __restrict__ scale, int64_t scale_ld) {
   pdl_wait();  // the previous kernel of the stream has completed
@@ -657,6 +659,249 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Fp8Shape<2>::THREADS
 }
 
 // ---------------------------------------------------------------------------
+// Few rows: the weight is streamed once through the registers.
+//
+// With at most 8 rows per weight the product is the time to read the weight,
+// and a 128-row MMA tile leaves most SMs without a tile (4096 x 4096: 16 tiles).
+// Here a CTA takes 16 weight rows and its warps share the k-blocks: a lane holds
+// 2 rows x 2 x 16 bytes of a block, which are the A operand of four
+// mma.m16n8k32 as they are (both operands use the same order of the 128
+// columns, so no lane exchanges bytes), and quantizes the 32 columns of its
+// activation row that it needs as the B operand itself: the block's largest
+// magnitude is two shuffles among four lanes. All loads of FP8_AHEAD blocks are
+// issued before the first product.
+//
+// Up  (SwiGLU): gate and up rows together, h = swiglu kept in fp32.
+// Down (routed): each warp takes one of the token's routed slots (or a share of
+// its k-blocks) and the sum over the warps is the weighted combine.
+// ---------------------------------------------------------------------------
+enum Fp8Stream : int { FP8_STREAM_LINEAR = 0, FP8_STREAM_UP = 1, FP8_STREAM_DOWN = 2 };
+
+struct Fp8StreamParams {
+  const void* x;          // LINEAR, UP: bf16 rows, pitch ldx; DOWN: fp32 hidden rows [rows or rows * top_k, K]
+  int64_t ldx;
+  const uint8_t* wq;      // [E][N][K]
+  const float* ws;        // [E][N blocks][K blocks]
+  int32_t rows;           // rows of x (tokens)
+  int32_t N, K;           // UP: N = 2F
+  int32_t experts;
+  int32_t top_k;          // 0: dense (all rows share the weight); else one row per routed slot
+  const int64_t* top_idx;
+  const uint16_t* gate;   // DOWN, routed
+  float scaling;
+  const uint16_t* shared;  // DOWN, routed: added after rounding, or nullptr
+  float* hidden;          // UP: [rows or rows * top_k, F]
+  uint16_t* out;          // LINEAR, DOWN: bf16 [rows, N]
+};
+
+constexpr int kFp8StreamWarps = 8;
+
+// Sixteen activations of a row as floats.
+__device__ __forceinline__ void load16(const uint16_t* p, float (&v)[16]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint4 u = __ldg(reinterpret_cast<const uint4*>(p) + i);
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = unpack_bf16x2(w[j]);
+      v[8 * i + 2 * j] = f.x;
+      v[8 * i + 2 * j + 1] = f.y;
+    }
+  }
+}
+__device__ __forceinline__ void load16(const float* p, float (&v)[16]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float4 f = __ldg(reinterpret_cast<const float4*>(p) + i);
+    v[4 * i] = f.x;
+    v[4 * i + 1] = f.y;
+    v[4 * i + 2] = f.z;
+    v[4 * i + 3] = f.w;
+  }
+}
+
+// d += A (16 x 32 E4M3) * B (32 x 8 E4M3), fp32 sums
+__device__ __forceinline__ void mma_e4m3_16x8x32(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                                 uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// 16 weight rows from w (row pitch k, `live` of them) times the activation row
+// of this lane's group (lanes 4 g .. 4 g + 3 hold row g; xrow null: none), over
+// the k-blocks kb0, kb0 + step, ..: acc[i][0..3] += rows (g, g + 8) x activation
+// rows (2 t, 2 t + 1). SETS = 2: a second set of 16 rows at w + set_off, its
+// scales at ws + ws_off.
+template <int SETS, typename T>
+__device__ __forceinline__ void fp8_stream_blocks(const T* xrow, const uint8_t* w, int64_t set_off, int live,
+                                                  const float* ws, int64_t ws_off, int k, int kb0, int step,
+                                                  float (&acc)[SETS][4]) {
+  constexpr int kAhead = 4 / SETS;  // k-blocks whose loads are in flight
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int k_blocks = (k + kFp8Block - 1) / kFp8Block;
+  const uint8_t* wr = w + (int64_t)g * k + 16 * t;
+  for (int base = kb0; base < k_blocks; base += kAhead * step) {
+    uint4 a[kAhead][SETS][2][2];  // [block][set][row g, g + 8][64-byte half]
+    float sw[kAhead][SETS];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int kb = base + i * step;
+#pragma unroll
+      for (int s = 0; s < SETS; ++s) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int col = kb * kFp8Block + 64 * j + 16 * t;
+            a[i][s][r][j] = make_uint4(0u, 0u, 0u, 0u);
+            if (kb < k_blocks && col < k && g + 8 * r < live)
+              a[i][s][r][j] = ldg_stream(reinterpret_cast<const uint4*>(
+                  wr + s * set_off + (int64_t)8 * r * k + kb * kFp8Block + 64 * j));
+          }
+        sw[i][s] = kb < k_blocks ? __ldg(ws + s * ws_off + kb) : 0.0f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int kb = base + i * step;
+      if (kb >= k_blocks) break;
+      float v[2][16];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int col = kb * kFp8Block + 64 * j + 16 * t;
+        if (xrow != nullptr && col < k) {
+          load16(xrow + col, v[j]);
+        } else {
+#pragma unroll
+          for (int q = 0; q < 16; ++q) v[j][q] = 0.0f;
+        }
+      }
+      float m = kFp8MinAmax;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int q = 0; q < 16; ++q) m = fmaxf(m, fabsf(v[j][q]));
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+      const float r = div_rn(kE4m3Max, m), sx = div_rn(m, kE4m3Max);
+      uint32_t b[2][4];
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          b[j][q] = cvt_e4m3x4(mul_rn(v[j][4 * q], r), mul_rn(v[j][4 * q + 1], r), mul_rn(v[j][4 * q + 2], r),
+                               mul_rn(v[j][4 * q + 3], r));
+      const float s0 = __shfl_sync(0xffffffffu, sx, 8 * t), s1 = __shfl_sync(0xffffffffu, sx, 8 * t + 4);
+#pragma unroll
+      for (int s = 0; s < SETS; ++s) {
+        float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const uint4 lo = a[i][s][0][j], hi = a[i][s][1][j];
+          mma_e4m3_16x8x32(d, lo.x, hi.x, lo.y, hi.y, b[j][0], b[j][1]);
+          mma_e4m3_16x8x32(d, lo.z, hi.z, lo.w, hi.w, b[j][2], b[j][3]);
+        }
+        const float f0 = s0 * sw[i][s], f1 = s1 * sw[i][s];
+        acc[s][0] = fmaf(d[0], f0, acc[s][0]);
+        acc[s][1] = fmaf(d[1], f1, acc[s][1]);
+        acc[s][2] = fmaf(d[2], f0, acc[s][2]);
+        acc[s][3] = fmaf(d[3], f1, acc[s][3]);
+      }
+    }
+  }
+}
+
+// blockIdx.x: 16 weight rows (UP: 16 hidden columns); blockIdx.y: dense: 0;
+// UP: the routed slot; DOWN: the token.
+template <int OP>
+__global__ void __launch_bounds__(32 * kFp8StreamWarps) fp8_stream_kernel(const __grid_constant__ Fp8StreamParams p) {
+  pdl_wait();  // the previous kernel of the stream has completed
+  pdl_trigger();
+  constexpr int SETS = OP == FP8_STREAM_UP ? 2 : 1;
+  using T = typename std::conditional<OP == FP8_STREAM_DOWN, float, uint16_t>::type;
+  __shared__ float s_sum[kFp8StreamWarps][SETS][16][8];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int n0 = blockIdx.x * 16;
+  const int rows_n = OP == FP8_STREAM_UP ? p.N / 2 : p.N;  // output columns
+  const int k_blocks = (p.K + kFp8Block - 1) / kFp8Block, n_blocks = (p.N + kFp8Block - 1) / kFp8Block;
+  const bool routed = p.top_k > 0;
+  int expert = 0, kb0 = warp, step = kFp8StreamWarps;
+  bool busy = true;
+  float weight = 1.0f;
+  const T* xrow = nullptr;
+  if (!routed) {
+    if (g < p.rows) xrow = static_cast<const T*>(p.x) + (int64_t)g * p.ldx;
+  } else if (OP == FP8_STREAM_DOWN) {
+    // warps per slot, as many as fit
+    const int per = kFp8StreamWarps / p.top_k, slot = warp / per;
+    busy = slot < p.top_k;
+    if (busy) {
+      const int64_t r = (int64_t)blockIdx.y * p.top_k + slot;
+      expert = checked_expert(p.top_idx[r], p.experts);
+      weight = mul_rn(bf16_to_f32(p.gate[r]), p.scaling);
+      kb0 = warp % per;
+      step = per;
+      if (g == 0) xrow = static_cast<const T*>(p.x) + r * p.ldx;
+    }
+  } else {
+    expert = checked_expert(p.top_idx[blockIdx.y], p.experts);
+    if (g == 0) xrow = static_cast<const T*>(p.x) + (int64_t)(blockIdx.y / p.top_k) * p.ldx;
+  }
+  float acc[SETS][4] = {};
+  if (busy) {
+    const uint8_t* w = p.wq + ((int64_t)expert * p.N + n0) * p.K;
+    const float* ws = p.ws + ((int64_t)expert * n_blocks + n0 / kFp8Block) * k_blocks;
+    fp8_stream_blocks<SETS, T>(xrow, w, (int64_t)rows_n * p.K, rows_n - n0, ws,
+                               (int64_t)(rows_n / kFp8Block) * k_blocks, p.K, kb0, step, acc);
+  }
+#pragma unroll
+  for (int s = 0; s < SETS; ++s) {
+    s_sum[warp][s][g][2 * t] = acc[s][0] * weight;
+    s_sum[warp][s][g][2 * t + 1] = acc[s][1] * weight;
+    s_sum[warp][s][g + 8][2 * t] = acc[s][2] * weight;
+    s_sum[warp][s][g + 8][2 * t + 1] = acc[s][3] * weight;
+  }
+  __syncthreads();
+  if (threadIdx.x >= 128) return;
+  const int n = threadIdx.x & 15, c = threadIdx.x >> 4;  // output column n0 + n of activation row c
+  if (c >= (routed ? 1 : p.rows) || n0 + n >= rows_n) return;
+  float sum[SETS];
+#pragma unroll
+  for (int s = 0; s < SETS; ++s) {
+    sum[s] = s_sum[0][s][n][c];
+#pragma unroll
+    for (int i = 1; i < kFp8StreamWarps; ++i) sum[s] += s_sum[i][s][n][c];
+  }
+  const int64_t row = routed ? blockIdx.y : c;
+  if constexpr (OP == FP8_STREAM_UP) {
+    float g0 = sum[0], g1 = 0.0f;
+    swiglu_pair_f32(g0, g1, sum[1], 0.0f);
+    p.hidden[row * rows_n + n0 + n] = g0;
+  } else {
+    uint16_t y = f32_to_bf16(sum[0]);
+    if (OP == FP8_STREAM_DOWN && routed && p.shared != nullptr)
+      y = f32_to_bf16(add_rn(bf16_to_f32(y), bf16_to_f32(p.shared[row * rows_n + n0 + n])));
+    p.out[row * rows_n + n0 + n] = y;
+  }
+}
+
+// The dispatch of `rows` rows to themselves (one expert, gate 1), for the fused
+// tail after a streamed feed-forward.
+__global__ void fp8_identity_kernel(int rows, int64_t* inverse, int64_t* top_idx, uint16_t* gate, int32_t* csr,
+                                    int32_t* pcsr) {
+  pdl_wait();  // the previous kernel of the stream has completed
+  pdl_trigger();
+  for (int i = threadIdx.x; i < rows; i += blockDim.x) {
+    inverse[i] = i;
+    top_idx[i] = 0;
+    gate[i] = 0x3F80;  // 1 in bf16
+  }
+  if (threadIdx.x < 2) csr[threadIdx.x] = pcsr[threadIdx.x] = threadIdx.x == 0 ? 0 : rows;
+}
+
+// ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
 // Rows of `cols` elements in boxes of 128 bytes x box_rows, 128-byte swizzle.
@@ -795,6 +1040,45 @@ int run_fp8_gemm(const Fp8Gemm& g, cudaStream_t stream) {
   if (swiglu)
     return pair ? fp8_launch<2, FP8_SWIGLU>(p, units, stream) : fp8_launch<1, FP8_SWIGLU>(p, units, stream);
   return pair ? fp8_launch<2, FP8_PLAIN>(p, units, stream) : fp8_launch<1, FP8_PLAIN>(p, units, stream);
+}
+
+template <int OP>
+static int fp8_stream_launch(const Fp8StreamParams& p, int groups, cudaStream_t stream) {
+  const int cols = OP == FP8_STREAM_UP ? p.N / 2 : p.N;
+  launch_pdl(fp8_stream_kernel<OP>, dim3((unsigned)((cols + 15) / 16), (unsigned)groups), dim3(32 * kFp8StreamWarps), 0,
+             stream, p);
+  return check_launch("fp8_stream");
+}
+
+// Whether a product of `rows` rows goes through the streaming kernels: dense up
+// to the 8 rows that share a weight; routed slots read their expert's weight
+// each for itself, so as long as they are few.
+static bool fp8_streams(int64_t rows, int top_k, int experts) {
+  return top_k == 0 ? rows <= 8 : rows * top_k <= 16 || rows * top_k <= (experts < 64 ? experts : 64);
+}
+
+static int run_fp8_stream_linear(const Fp8StreamParams& p, cudaStream_t stream) {
+  return fp8_stream_launch<FP8_STREAM_LINEAR>(p, 1, stream);
+}
+
+// The feed-forward: p.x bf16 rows, p.hidden fp32 scratch.
+static int run_fp8_stream_ffn(Fp8StreamParams p, const uint8_t* down_q, const float* down_scale, int32_t dim,
+                              int32_t hidden, cudaStream_t stream) {
+  int rc = fp8_stream_launch<FP8_STREAM_UP>(p, p.top_k > 0 ? p.rows * p.top_k : 1, stream);
+  if (rc) return rc;
+  p.x = p.hidden;
+  p.ldx = hidden;
+  p.wq = down_q;
+  p.ws = down_scale;
+  p.N = dim;
+  p.K = hidden;
+  return fp8_stream_launch<FP8_STREAM_DOWN>(p, p.top_k > 0 ? p.rows : 1, stream);
+}
+
+static int run_fp8_identity(int rows, int64_t* inverse, int64_t* top_idx, uint16_t* gate, int32_t* csr, int32_t* pcsr,
+                            cudaStream_t stream) {
+  launch_pdl(fp8_identity_kernel, dim3(1), dim3(64), 0, stream, rows, inverse, top_idx, gate, csr, pcsr);
+  return check_launch("fp8_identity");
 }
 
 }  // namespace praxis

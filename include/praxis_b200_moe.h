@@ -437,7 +437,8 @@ int praxis_b200_fp8_pack_weights(const void* w, int32_t experts, int32_t k, int3
 
 /* out [rows, n] bf16 = x [rows, k] (bf16, row pitch ldx) times the transposed
  * weight w_q [n, k], w_scale [ceil(n / 128), ceil(k / 128)]. k % 16 == 0,
- * ldx % 8 == 0, any n; x and w_q 16-byte aligned. */
+ * ldx % 8 == 0, any n; x and w_q 16-byte aligned. A workspace size of 0 needs
+ * no workspace (few rows). */
 size_t praxis_b200_fp8_linear_workspace_size(int64_t rows, int32_t n, int32_t k);
 int praxis_b200_fp8_linear(const void* x, int64_t rows, int32_t k, int64_t ldx, const void* w_q, const float* w_scale,
                            int32_t n, void* out, void* workspace, size_t workspace_size, int device, void* stream);

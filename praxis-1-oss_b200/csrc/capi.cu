@@ -748,7 +748,7 @@ int praxis_b200_fp8_pack_weights(const void* w, int32_t experts, int32_t k, int3
 
 size_t praxis_b200_fp8_linear_workspace_size(int64_t rows, int32_t n, int32_t k) {
   (void)n;
-  return rows < 0 || k < 0 ? 0 : fp8_linear_layout(rows, k).total;
+  return rows < 0 || k < 0 || fp8_streams(rows, 0, 1) ? 0 : fp8_linear_layout(rows, k).total;
 }
 
 int praxis_b200_fp8_linear(const void* x, int64_t rows, int32_t k, int64_t ldx, const void* w_q, const float* w_scale,
@@ -757,14 +757,12 @@ int praxis_b200_fp8_linear(const void* x, int64_t rows, int32_t k, int64_t ldx, 
   int rc = fp8_check("fp8_linear", rows, n, k);
   if (rc) return rc;
   if (rows == 0) return PRAXIS_B200_OK;
-  if (!x || !w_q || !w_scale || !out || !workspace) return set_error(PRAXIS_B200_EINVAL, "fp8_linear: null pointer");
+  const bool streams = fp8_streams(rows, 0, 1);
+  if (!x || !w_q || !w_scale || !out || (!streams && !workspace)) return set_error(PRAXIS_B200_EINVAL, "fp8_linear: null pointer");
   if (ldx < k || ldx % 8 != 0 || (((uintptr_t)x | (uintptr_t)w_q | (uintptr_t)workspace) & 15) || ((uintptr_t)out & 1))
     return set_error(PRAXIS_B200_EINVAL, "fp8_linear: row pitch or alignment");
-  const Fp8LinearLayout L = fp8_linear_layout(rows, k);
-  if (workspace_size < L.total)
-    return set_error(PRAXIS_B200_EINVAL, "fp8_linear: workspace %zu < %zu bytes", workspace_size, L.total);
   cudaStream_t s = PRAXIS_STREAM(stream);
-  if (fp8_streams(rows, 0, 1)) {
+  if (streams) {
     Fp8StreamParams p = {};
     p.x = x;
     p.ldx = ldx;
@@ -777,6 +775,9 @@ int praxis_b200_fp8_linear(const void* x, int64_t rows, int32_t k, int64_t ldx, 
     p.out = static_cast<uint16_t*>(out);
     return run_fp8_stream_linear(p, s);
   }
+  const Fp8LinearLayout L = fp8_linear_layout(rows, k);
+  if (workspace_size < L.total)
+    return set_error(PRAXIS_B200_EINVAL, "fp8_linear: workspace %zu < %zu bytes", workspace_size, L.total);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   float* scale = reinterpret_cast<float*>(ws + L.scale);
   rc = run_fp8_quantize(static_cast<const uint16_t*>(x), rows, k, ldx, kFp8SameRows, ws + L.q, scale, L.scale_ld, s);

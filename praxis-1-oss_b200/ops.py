@@ -37,7 +37,7 @@ def _stream(t: Tensor) -> C.c_void_p:
 
 
 def _need(t: Tensor, name: str, dtype, ndim: int | None = None, device=None) -> None:
-    if not isinstance(t, Tensor) or t.dtype != dtype or not t.is_contiguous() or t.device.type != "cuda":
+    if not isinstance(t, Tensor) or t.dtype != dtype or not t.is_contiguous() or not t.is_cuda:
         raise ValueError(f"{name}: expected a contiguous CUDA {dtype} tensor")
     if ndim is not None and t.ndim != ndim:
         raise ValueError(f"{name}: expected {ndim} dims, got {t.ndim}")
@@ -49,14 +49,21 @@ _ACTIVATIONS = {"sigmoid": capi.SIGMOID, "softmax": capi.SOFTMAX}
 _GROUP_SCORES = {"top2": capi.GROUP_TOP2, "max": capi.GROUP_MAX}
 
 
-def _run(t: Tensor, fn, *args) -> None:
-    """Calls a C entry point, which makes ``t``'s device current, and gives
-    the caller its current device back."""
-    device = torch.cuda.current_device()
+def _run(device: int, fn, *args) -> None:
+    """Calls a C entry point, which makes ``device`` current, and gives the
+    caller its current device back."""
+    current = torch._C._cuda_getDevice()
     status = fn(*args)
-    if t.device.index != device:
-        torch.cuda.set_device(device)
-    capi.check(status)
+    if device != current:
+        torch.cuda.set_device(current)
+    if status:
+        capi.check(status)
+
+
+def _place(t: Tensor) -> tuple[int, int]:
+    """(device ordinal, its current stream) of a CUDA tensor."""
+    device = t.get_device()
+    return device, torch._C._cuda_getCurrentRawStream(device)
 
 
 def padded_rows(routed_rows: int, experts: int) -> int:
@@ -144,15 +151,17 @@ def route(logits: Tensor, bias: Tensor | None, top_k: int, activation: str = "si
                         or top_k > top_groups * (e // groups)):
         raise ValueError("group-limited routing needs 1..32 equal groups, 1 <= top_groups <= groups and top_k within "
                          "the experts of the open groups")
-    top_idx = torch.empty(t, top_k, dtype=torch.int64, device=logits.device)
-    gate = torch.empty(t, top_k, dtype=BF16, device=logits.device)
+    top_idx = logits.new_empty((t, top_k), dtype=torch.int64)
+    gate = logits.new_empty((t, top_k), dtype=BF16)
     lib = capi.load()
     if groups == 1:
         capi.check(lib.praxis_b200_route(
             _p(logits), _p(bias), t, e, top_k, act, _p(top_idx), _p(gate), _dev(logits), _stream(logits)))
         return top_idx, gate
-    _run(logits, lib.praxis_b200_route_groups, _p(logits), _p(bias), t, e, top_k, act, groups, top_groups,
-         _GROUP_SCORES[group_score], _p(top_idx), _p(gate), _dev(logits), _stream(logits))
+    device, stream = _place(logits)
+    _run(device, lib.praxis_b200_route_groups, logits.data_ptr(), None if bias is None else bias.data_ptr(), t, e,
+         top_k, act, groups, top_groups, _GROUP_SCORES[group_score], top_idx.data_ptr(), gate.data_ptr(), device,
+         stream)
     return top_idx, gate
 
 
@@ -713,34 +722,46 @@ def moe_forward(x: Tensor, top_idx: Tensor | None, gate: Tensor | None, gate_up_
 
 
 # -- block-scaled FP8 weights ------------------------------------------------
-def _fp8_weight(q: Tensor, scale: Tensor, name: str, ndim: int, device) -> None:
+def _fp8_weight(q: Tensor, scale: Tensor, name: str, ndim: int) -> None:
     """E4M3 values [.., N, K] with one fp32 scale per 128 x 128 block."""
-    _need(q, name + "_q", F8, ndim, device)
-    _need(scale, name + "_scale", torch.float32, ndim, device)
-    n, k = q.shape[-2:]
-    want = q.shape[:-2] + (-(-n // 128), -(-k // 128))
-    if scale.shape != want:
-        raise ValueError(f"{name}_scale: expected {tuple(want)}, got {tuple(scale.shape)}")
+    _need(q, name + "_q", F8, ndim)
+    _need(scale, name + "_scale", torch.float32, ndim)
+    _same_device(q, scale)
+    shape = q.shape
+    if shape[:-2] + (-(-shape[-2] // 128), -(-shape[-1] // 128)) != scale.shape:
+        raise ValueError(f"{name}_scale: got {tuple(scale.shape)}, expected one scale per 128 x 128 block of "
+                         f"{tuple(shape)}")
 
 
-def _fp8_rows(x: Tensor, width: int) -> Tensor:
-    """x [.., width] as bf16 rows whose columns are neighbours."""
-    if not isinstance(x, Tensor) or x.dtype != BF16 or x.device.type != "cuda" or x.ndim < 1:
+def _fp8_rows(x: Tensor, width: int) -> tuple[Tensor, int, int]:
+    """x [.., width] as (bf16 rows whose columns are neighbours, their number
+    and their pitch)."""
+    if not isinstance(x, Tensor) or x.dtype is not BF16 or not x.is_cuda or x.ndim < 1:
         raise ValueError("x: expected a CUDA bf16 tensor")
     if x.shape[-1] != width:
         raise ValueError(f"x: expected {width} columns, got {x.shape[-1]}")
-    if x.ndim != 2:
-        if not x.is_contiguous():
-            raise ValueError("x: expected a contiguous tensor or rows of one pitch")
-        x = x.view(-1, width)
-    if x.numel() and (x.stride(1) != 1 or (x.shape[0] > 1 and (x.stride(0) < width or x.stride(0) % 8))
-                      or x.data_ptr() % 16):
-        raise ValueError("x: rows must be contiguous, 16-byte aligned and a multiple of 8 elements apart")
-    return x
+    if x.is_contiguous():
+        rows, pitch = x.numel() // width if width else 0, width
+    elif x.ndim != 2:
+        raise ValueError("x: expected a contiguous tensor or rows of one pitch")
+    else:
+        rows = x.shape[0]
+        pitch = x.stride(0) if rows > 1 else width
+        if x.stride(1) != 1 or pitch < width or pitch % 8:
+            raise ValueError("x: rows must be contiguous and a multiple of 8 elements apart")
+    return x, rows, pitch
 
 
-def _pitch(x: Tensor) -> int:
-    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+def _same_device(x: Tensor, *others) -> None:
+    device = x.get_device()
+    for t in others:
+        if t is not None and t.get_device() != device:
+            raise ValueError("tensors must share a device")
+
+
+def _inference_only(*tensors) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError("the FP8 products support inference only")
 
 
 def fp8_quantize(x: Tensor) -> tuple[Tensor, Tensor]:
@@ -750,12 +771,14 @@ def fp8_quantize(x: Tensor) -> tuple[Tensor, Tensor]:
     e4m3(x * f32(448 / a)) with scale f32(a / 448)."""
     if not isinstance(x, Tensor) or x.ndim != 2:
         raise ValueError("x: expected 2 dims")
-    x = _fp8_rows(x, x.shape[1])
-    r, k = x.shape
+    k = x.shape[1]
+    x, r, pitch = _fp8_rows(x, k)
     ld = -(-max(r, 1) // 32) * 32
     q = torch.empty(r, k, dtype=F8, device=x.device)
     scale = torch.empty(-(-k // 128), ld, dtype=torch.float32, device=x.device)
-    _run(x, capi.load().praxis_b200_fp8_quantize, _p(x), r, k, _pitch(x), _p(q), _p(scale), ld, _dev(x), _stream(x))
+    device, stream = _place(x)
+    _run(device, capi.load().praxis_b200_fp8_quantize, x.data_ptr(), r, k, pitch, q.data_ptr(), scale.data_ptr(), ld,
+         device, stream)
     return q, scale[:, :r].T
 
 
@@ -770,7 +793,9 @@ def fp8_pack_weights(w: Tensor) -> tuple[Tensor, Tensor]:
     k, n = w.shape[-2:]
     q = torch.empty(w.shape[:-2] + (n, k), dtype=F8, device=w.device)
     scale = torch.empty(w.shape[:-2] + (-(-n // 128), -(-k // 128)), dtype=torch.float32, device=w.device)
-    _run(w, capi.load().praxis_b200_fp8_pack_weights, _p(w), e, k, n, _p(q), _p(scale), _dev(w), _stream(w))
+    device, stream = _place(w)
+    _run(device, capi.load().praxis_b200_fp8_pack_weights, w.data_ptr(), e, k, n, q.data_ptr(), scale.data_ptr(),
+         device, stream)
     return q, scale
 
 
@@ -780,37 +805,27 @@ def fp8_linear(x: Tensor, w_q: Tensor, w_scale: Tensor) -> Tensor:
     x [.., K] bf16 (2-D rows may be a column slice of a wider tensor) is
     quantized in the call as by :func:`fp8_quantize`; the products are summed
     in fp32. K % 16 == 0, any N, any number of rows. Inference only."""
-    _fp8_weight(w_q, w_scale, "w", 2, None)
+    _fp8_weight(w_q, w_scale, "w", 2)
     n, k = w_q.shape
-    rows = _fp8_rows(x, k)
-    _same_device(x, w_q, w_scale)
+    x, r, pitch = _fp8_rows(x, k)
+    _same_device(x, w_q)
     _inference_only(x)
-    r = rows.shape[0]
-    out = torch.empty(x.shape[:-1] + (n,), dtype=BF16, device=x.device)
+    out = x.new_empty(x.shape[:-1] + (n,))
     lib = capi.load()
-    size = int(lib.praxis_b200_fp8_linear_workspace_size(r, n, k))
-    ws = torch.empty(size, dtype=torch.uint8, device=x.device)
-    _run(x, lib.praxis_b200_fp8_linear, _p(rows), r, k, _pitch(rows), _p(w_q), _p(w_scale), n, _p(out), _p(ws), size,
-         _dev(x), _stream(x))
+    size = lib.praxis_b200_fp8_linear_workspace_size(r, n, k)
+    ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
+    device, stream = _place(x)
+    _run(device, lib.praxis_b200_fp8_linear, x.data_ptr(), r, k, pitch, w_q.data_ptr(), w_scale.data_ptr(), n,
+         out.data_ptr(), None if ws is None else ws.data_ptr(), size, device, stream)
     return out
-
-
-def _same_device(x: Tensor, *others) -> None:
-    if any(t is not None and t.device != x.device for t in others):
-        raise ValueError("tensors must share a device")
-
-
-def _inference_only(*tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError("the FP8 products support inference only")
 
 
 def _fp8_ffn_shapes(gate_up_q: Tensor, gate_up_scale: Tensor, down_q: Tensor, down_scale: Tensor, ndim: int
                     ) -> tuple[int, int, int]:
     """(E, C, F) of a gate/up and a down weight that belong together."""
-    _fp8_weight(gate_up_q, gate_up_scale, "gate_up", ndim, None)
-    _fp8_weight(down_q, down_scale, "down", ndim, gate_up_q.device)
-    _same_device(gate_up_q, gate_up_scale, down_scale)
+    _fp8_weight(gate_up_q, gate_up_scale, "gate_up", ndim)
+    _fp8_weight(down_q, down_scale, "down", ndim)
+    _same_device(gate_up_q, down_q)
     f2, c = gate_up_q.shape[-2:]
     f = f2 // 2
     if f2 % 2 or c % 128 or f % 128 or not c or not f or down_q.shape != gate_up_q.shape[:-2] + (c, f):
@@ -818,23 +833,24 @@ def _fp8_ffn_shapes(gate_up_q: Tensor, gate_up_scale: Tensor, down_q: Tensor, do
     return (gate_up_q.shape[0] if ndim == 3 else 1), c, f
 
 
-def _fp8_ffn(rows: Tensor, top_idx: Tensor | None, gate: Tensor | None, shared: Tensor | None, out: Tensor | None,
+def _ptr(t: Tensor | None):
+    return None if t is None else t.data_ptr()
+
+
+def _fp8_ffn(x: Tensor, t: int, top_idx: Tensor | None, gate: Tensor | None, shared: Tensor | None, out: Tensor | None,
              weights: tuple, sizes: tuple, scaling: float, tail=None) -> None:
     e, c, f = sizes
-    t = rows.shape[0]
     k = 0 if top_idx is None else top_idx.shape[1]
     lib = capi.load()
-    size = int(lib.praxis_b200_fp8_ffn_workspace_size(t, k, e, c, f))
-    ws = torch.empty(size, dtype=torch.uint8, device=rows.device)
+    size = lib.praxis_b200_fp8_ffn_workspace_size(t, k, e, c, f)
+    ws = torch.empty(size, dtype=torch.uint8, device=x.device)
     gate_up_q, gate_up_scale, down_q, down_scale = weights
-    args = capi.Fp8FfnArgs(
-        x=rows.data_ptr(), top_idx=_p(top_idx), gate=_p(gate), shared=_p(shared), out=_p(out),
-        gate_up_q=gate_up_q.data_ptr(), gate_up_scale=gate_up_scale.data_ptr(), down_q=down_q.data_ptr(),
-        down_scale=down_scale.data_ptr(), tokens=t, dim=c, hidden=f, experts=e, top_k=k, scaling=float(scaling),
-        workspace=ws.data_ptr(), workspace_size=size, device=_dev(rows),
-        stream=torch.cuda.current_stream(rows.device).cuda_stream,
-        tail=None if tail is None else C.addressof(tail))
-    _run(rows, lib.praxis_b200_fp8_ffn, C.byref(args))
+    device, stream = _place(x)
+    args = capi.Fp8FfnArgs(  # in the order of the struct
+        x.data_ptr(), _ptr(top_idx), _ptr(gate), _ptr(shared), _ptr(out), gate_up_q.data_ptr(),
+        gate_up_scale.data_ptr(), down_q.data_ptr(), down_scale.data_ptr(), t, c, f, e, k, scaling, ws.data_ptr(),
+        size, device, stream, None if tail is None else C.addressof(tail))
+    _run(device, lib.praxis_b200_fp8_ffn, C.byref(args))
 
 
 def fp8_mlp(x: Tensor, gate_up_q: Tensor, gate_up_scale: Tensor, down_q: Tensor, down_scale: Tensor, *,
@@ -845,9 +861,9 @@ def fp8_mlp(x: Tensor, gate_up_q: Tensor, gate_up_scale: Tensor, down_q: Tensor,
     their activations (:func:`fp8_quantize`); the hidden values go from fp32
     to E4M3 without a rounding in between. Inference only."""
     sizes = _fp8_ffn_shapes(gate_up_q, gate_up_scale, down_q, down_scale, 2)
-    if not isinstance(x, Tensor) or not x.is_contiguous():
+    x, t, pitch = _fp8_rows(x, sizes[1])
+    if pitch != sizes[1]:
         raise ValueError("x: expected a contiguous CUDA bf16 tensor")
-    rows = _fp8_rows(x, sizes[1])
     _same_device(x, gate_up_q)
     _inference_only(x)
     if out is None:
@@ -856,7 +872,7 @@ def fp8_mlp(x: Tensor, gate_up_q: Tensor, gate_up_scale: Tensor, down_q: Tensor,
         _need(out, "out", BF16, x.ndim, x.device)
         if out.shape != x.shape:
             raise ValueError("out must have the shape of x")
-    _fp8_ffn(rows, None, None, None, out, (gate_up_q, gate_up_scale, down_q, down_scale), sizes, 1.0)
+    _fp8_ffn(x, t, None, None, None, out, (gate_up_q, gate_up_scale, down_q, down_scale), sizes, 1.0)
     return out
 
 
@@ -871,23 +887,24 @@ def fp8_moe_forward(x: Tensor, top_idx: Tensor, gate: Tensor, gate_up_q: Tensor,
     residual, normed rows or None)`` as there. Inference only."""
     sizes = _fp8_ffn_shapes(gate_up_q, gate_up_scale, down_q, down_scale, 3)
     e, c, _ = sizes
-    _need(x, "x", BF16, 2, gate_up_q.device)
+    _need(x, "x", BF16, 2)
     t = x.shape[0]
     if x.shape[1] != c:
         raise ValueError(f"x: expected {c} columns, got {x.shape[1]}")
-    _need(top_idx, "top_idx", torch.int64, 2, x.device)
-    _need(gate, "gate", BF16, 2, x.device)
+    _need(top_idx, "top_idx", torch.int64, 2)
+    _need(gate, "gate", BF16, 2)
     if top_idx.shape[0] != t or gate.shape != top_idx.shape or not 1 <= top_idx.shape[1] <= min(8, e):
         raise ValueError("top_idx / gate: expected [T, k], 1 <= k <= min(8, E)")
     if shared is not None:
-        _need(shared, "shared", BF16, 2, x.device)
+        _need(shared, "shared", BF16, 2)
         if shared.shape != x.shape:
             raise ValueError("shared must have the shape of x")
+    _same_device(x, gate_up_q, top_idx, gate, shared)
     _inference_only(x, gate, shared)
     weights = (gate_up_q, gate_up_scale, down_q, down_scale)
     if tail is not None:
         st, residual_out, normed = _tail_struct(tail, t, c, x.device, tail_out)
-        _fp8_ffn(x, top_idx, gate, shared, None, weights, sizes, scaling, st)
+        _fp8_ffn(x, t, top_idx, gate, shared, None, weights, sizes, float(scaling), st)
         return residual_out, normed
     if out is None:
         out = torch.empty_like(x)
@@ -895,5 +912,5 @@ def fp8_moe_forward(x: Tensor, top_idx: Tensor, gate: Tensor, gate_up_q: Tensor,
         _need(out, "out", BF16, 2, x.device)
         if out.shape != x.shape:
             raise ValueError("out must have the shape of x")
-    _fp8_ffn(x, top_idx, gate, shared, out, weights, sizes, scaling)
+    _fp8_ffn(x, t, top_idx, gate, shared, out, weights, sizes, float(scaling))
     return out

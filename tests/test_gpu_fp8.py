@@ -249,18 +249,20 @@ def test_linear_refuses_at_the_c_level(P):
     lib, p = P.capi.load(), P.ops._p
     g = gen(13)
     q, s = weight(g, 128, 256)
-    x = randn(g, 4, 256)
-    out = torch.empty(4, 128, dtype=BF16, device=DEV)
-    size = int(lib.praxis_b200_fp8_linear_workspace_size(4, 128, 256))
+    x = randn(g, 40, 256)
+    out = torch.empty(40, 128, dtype=BF16, device=DEV)
+    size = int(lib.praxis_b200_fp8_linear_workspace_size(40, 128, 256))
     ws = torch.empty(size, dtype=torch.uint8, device=DEV)
 
-    def call(rows=4, k=256, ldx=256, n=128, size=size, x=p(x)):
+    def call(rows=40, k=256, ldx=256, n=128, size=size, x=p(x)):
         return lib.praxis_b200_fp8_linear(x, rows, k, ldx, p(q), p(s), n, p(out), p(ws), size, 0, None)
 
     for kw in (dict(k=250), dict(ldx=252), dict(ldx=128), dict(n=0), dict(rows=-1), dict(size=size - 1), dict(x=None),
                dict(k=0)):
         assert call(**kw) == P.capi.EINVAL, kw
     assert call() == P.capi.OK
+    # up to 8 rows need no workspace
+    assert lib.praxis_b200_fp8_linear_workspace_size(8, 128, 256) == 0
     with pytest.raises(ValueError):
         P.ops.fp8_linear(randn(g, 4, 24), *weight(g, 128, 24))
 

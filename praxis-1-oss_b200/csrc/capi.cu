@@ -271,7 +271,7 @@ static Fp8FfnLayout fp8_ffn_layout(int64_t tokens, int top_k, int experts, int d
   L.stream_gate = take((size_t)tokens * 2);
   L.stream_csr = take(8);
   L.stream_pcsr = take(8);
-  if (fp8_streams(tokens, top_k, experts) && off > L.total) L.total = off;
+  if (fp8_streams(tokens, top_k, experts, dim, hidden) && off > L.total) L.total = off;
   return L;
 }
 
@@ -748,7 +748,7 @@ int praxis_b200_fp8_pack_weights(const void* w, int32_t experts, int32_t k, int3
 
 size_t praxis_b200_fp8_linear_workspace_size(int64_t rows, int32_t n, int32_t k) {
   (void)n;
-  return rows < 0 || k < 0 || fp8_streams(rows, 0, 1) ? 0 : fp8_linear_layout(rows, k).total;
+  return rows < 0 || k < 0 || fp8_streams(rows, 0, 1, k, 0) ? 0 : fp8_linear_layout(rows, k).total;
 }
 
 int praxis_b200_fp8_linear(const void* x, int64_t rows, int32_t k, int64_t ldx, const void* w_q, const float* w_scale,
@@ -757,7 +757,7 @@ int praxis_b200_fp8_linear(const void* x, int64_t rows, int32_t k, int64_t ldx, 
   int rc = fp8_check("fp8_linear", rows, n, k);
   if (rc) return rc;
   if (rows == 0) return PRAXIS_B200_OK;
-  const bool streams = fp8_streams(rows, 0, 1);
+  const bool streams = fp8_streams(rows, 0, 1, k, 0);
   if (!x || !w_q || !w_scale || !out || (!streams && !workspace)) return set_error(PRAXIS_B200_EINVAL, "fp8_linear: null pointer");
   if (ldx < k || ldx % 8 != 0 || (((uintptr_t)x | (uintptr_t)w_q | (uintptr_t)workspace) & 15) || ((uintptr_t)out & 1))
     return set_error(PRAXIS_B200_EINVAL, "fp8_linear: row pitch or alignment");
@@ -829,7 +829,7 @@ int praxis_b200_fp8_ffn(const praxis_b200_fp8_ffn_args* a) {
     return set_error(PRAXIS_B200_EINVAL, "fp8_ffn: workspace %zu < %zu bytes", a->workspace_size, L.total);
   cudaStream_t s = PRAXIS_STREAM(a->stream);
   uint8_t* ws = static_cast<uint8_t*>(a->workspace);
-  if (fp8_streams(a->tokens, top_k, a->experts)) {
+  if (fp8_streams(a->tokens, top_k, a->experts, a->dim, a->hidden)) {
     Fp8StreamParams p = {};
     p.x = a->x;
     p.ldx = a->dim;

@@ -666,10 +666,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Fp8Shape<2>::THREADS
 // Here a CTA takes 16 weight rows and its warps share the k-blocks: a lane holds
 // 2 rows x 2 x 16 bytes of a block, which are the A operand of four
 // mma.m16n8k32 as they are (both operands use the same order of the 128
-// columns, so no lane exchanges bytes), and quantizes the 32 columns of its
-// activation row that it needs as the B operand itself: the block's largest
-// magnitude is two shuffles among four lanes. All loads of FP8_AHEAD blocks are
-// issued before the first product.
+// columns, so no lane exchanges bytes). The CTA quantizes its activation rows
+// into shared memory while the first weight loads are in flight; a consumed
+// block's registers are loaded again at once.
 //
 // Up  (SwiGLU): gate and up rows together, h = swiglu kept in fp32.
 // Down (routed): each warp takes one of the token's routed slots (or a share of
@@ -694,30 +693,68 @@ struct Fp8StreamParams {
   uint16_t* out;          // LINEAR, DOWN: bf16 [rows, N]
 };
 
-constexpr int kFp8StreamWarps = 8;
+// DOWN has two warps for each of up to 8 slots.
+template <int OP>
+__host__ __device__ constexpr int fp8_stream_warps() {
+  return OP == FP8_STREAM_DOWN ? 16 : 8;
+}
 
-// Sixteen activations of a row as floats.
-__device__ __forceinline__ void load16(const uint16_t* p, float (&v)[16]) {
+// Quantized activation rows in shared memory: row pitch (64 bytes more than a
+// multiple of 128: the 8 rows of an operand load fall into different banks),
+// then the scales [rows][K blocks].
+__host__ __device__ constexpr int fp8_stream_pitch(int k) { return (k + kFp8Block - 1) / kFp8Block * kFp8Block + 64; }
+__host__ __device__ constexpr size_t fp8_stream_smem(int rows, int k) {
+  return (size_t)rows * (fp8_stream_pitch(k) + 4 * ((k + kFp8Block - 1) / kFp8Block));
+}
+
+// Eight activations of a row as floats.
+__device__ __forceinline__ void load8(const uint16_t* p, float (&v)[8]) {
+  const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const uint4 u = __ldg(reinterpret_cast<const uint4*>(p) + i);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float2 f = unpack_bf16x2(w[j]);
-      v[8 * i + 2 * j] = f.x;
-      v[8 * i + 2 * j + 1] = f.y;
-    }
+  for (int j = 0; j < 4; ++j) {
+    const float2 f = unpack_bf16x2(w[j]);
+    v[2 * j] = f.x;
+    v[2 * j + 1] = f.y;
   }
 }
-__device__ __forceinline__ void load16(const float* p, float (&v)[16]) {
+__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < 2; ++i) {
     const float4 f = __ldg(reinterpret_cast<const float4*>(p) + i);
     v[4 * i] = f.x;
     v[4 * i + 1] = f.y;
     v[4 * i + 2] = f.z;
     v[4 * i + 3] = f.w;
+  }
+}
+
+// `rows` rows (pitch ldx) -> codes and scales in shared memory, half a warp per
+// block of 128 columns. Columns past k are zero codes.
+template <typename T, int THREADS>
+__device__ __forceinline__ void fp8_stream_quantize(const T* x, int64_t ldx, int rows, int k, uint8_t* codes,
+                                                    float* scales) {
+  const int k_blocks = (k + kFp8Block - 1) / kFp8Block, pitch = fp8_stream_pitch(k);
+  const int total = rows * k_blocks, sub = threadIdx.x & 15;
+  for (int i0 = 0; i0 < total; i0 += THREADS / 16) {  // whole warps take every turn
+    const int i = i0 + (int)(threadIdx.x >> 4);
+    const int r = i / k_blocks, b = i - r * k_blocks, col = b * kFp8Block + 8 * sub;
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = 0.0f;
+    if (i < total && col < k) load8(x + (int64_t)r * ldx + col, v);
+    float m = kFp8MinAmax;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(v[j]));
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float q = div_rn(kE4m3Max, m);
+    if (i < total) {
+      *reinterpret_cast<uint2*>(codes + r * pitch + col) =
+          make_uint2(cvt_e4m3x4(mul_rn(v[0], q), mul_rn(v[1], q), mul_rn(v[2], q), mul_rn(v[3], q)),
+                     cvt_e4m3x4(mul_rn(v[4], q), mul_rn(v[5], q), mul_rn(v[6], q), mul_rn(v[7], q)));
+      if (sub == 0) scales[r * k_blocks + b] = div_rn(m, kE4m3Max);
+    }
   }
 }
 
@@ -729,113 +766,34 @@ __device__ __forceinline__ void mma_e4m3_16x8x32(float (&d)[4], uint32_t a0, uin
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// 16 weight rows from w (row pitch k, `live` of them) times the activation row
-// of this lane's group (lanes 4 g .. 4 g + 3 hold row g; xrow null: none), over
-// the k-blocks kb0, kb0 + step, ..: acc[i][0..3] += rows (g, g + 8) x activation
-// rows (2 t, 2 t + 1). SETS = 2: a second set of 16 rows at w + set_off, its
-// scales at ws + ws_off.
-template <int SETS, typename T>
-__device__ __forceinline__ void fp8_stream_blocks(const T* xrow, const uint8_t* w, int64_t set_off, int live,
-                                                  const float* ws, int64_t ws_off, int k, int kb0, int step,
-                                                  float (&acc)[SETS][4]) {
-  constexpr int kAhead = 4 / SETS;  // k-blocks whose loads are in flight
-  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int k_blocks = (k + kFp8Block - 1) / kFp8Block;
-  const uint8_t* wr = w + (int64_t)g * k + 16 * t;
-  for (int base = kb0; base < k_blocks; base += kAhead * step) {
-    uint4 a[kAhead][SETS][2][2];  // [block][set][row g, g + 8][64-byte half]
-    float sw[kAhead][SETS];
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      const int kb = base + i * step;
-#pragma unroll
-      for (int s = 0; s < SETS; ++s) {
-#pragma unroll
-        for (int r = 0; r < 2; ++r)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int col = kb * kFp8Block + 64 * j + 16 * t;
-            a[i][s][r][j] = make_uint4(0u, 0u, 0u, 0u);
-            if (kb < k_blocks && col < k && g + 8 * r < live)
-              a[i][s][r][j] = ldg_stream(reinterpret_cast<const uint4*>(
-                  wr + s * set_off + (int64_t)8 * r * k + kb * kFp8Block + 64 * j));
-          }
-        sw[i][s] = kb < k_blocks ? __ldg(ws + s * ws_off + kb) : 0.0f;
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      const int kb = base + i * step;
-      if (kb >= k_blocks) break;
-      float v[2][16];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int col = kb * kFp8Block + 64 * j + 16 * t;
-        if (xrow != nullptr && col < k) {
-          load16(xrow + col, v[j]);
-        } else {
-#pragma unroll
-          for (int q = 0; q < 16; ++q) v[j][q] = 0.0f;
-        }
-      }
-      float m = kFp8MinAmax;
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int q = 0; q < 16; ++q) m = fmaxf(m, fabsf(v[j][q]));
-      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-      const float r = div_rn(kE4m3Max, m), sx = div_rn(m, kE4m3Max);
-      uint32_t b[2][4];
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          b[j][q] = cvt_e4m3x4(mul_rn(v[j][4 * q], r), mul_rn(v[j][4 * q + 1], r), mul_rn(v[j][4 * q + 2], r),
-                               mul_rn(v[j][4 * q + 3], r));
-      const float s0 = __shfl_sync(0xffffffffu, sx, 8 * t), s1 = __shfl_sync(0xffffffffu, sx, 8 * t + 4);
-#pragma unroll
-      for (int s = 0; s < SETS; ++s) {
-        float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const uint4 lo = a[i][s][0][j], hi = a[i][s][1][j];
-          mma_e4m3_16x8x32(d, lo.x, hi.x, lo.y, hi.y, b[j][0], b[j][1]);
-          mma_e4m3_16x8x32(d, lo.z, hi.z, lo.w, hi.w, b[j][2], b[j][3]);
-        }
-        const float f0 = s0 * sw[i][s], f1 = s1 * sw[i][s];
-        acc[s][0] = fmaf(d[0], f0, acc[s][0]);
-        acc[s][1] = fmaf(d[1], f1, acc[s][1]);
-        acc[s][2] = fmaf(d[2], f0, acc[s][2]);
-        acc[s][3] = fmaf(d[3], f1, acc[s][3]);
-      }
-    }
-  }
-}
-
 // blockIdx.x: 16 weight rows (UP: 16 hidden columns); blockIdx.y: dense: 0;
 // UP: the routed slot; DOWN: the token.
 template <int OP>
-__global__ void __launch_bounds__(32 * kFp8StreamWarps) fp8_stream_kernel(const __grid_constant__ Fp8StreamParams p) {
+__global__ void __launch_bounds__(32 * fp8_stream_warps<OP>(), OP == FP8_STREAM_DOWN ? 1 : 2)
+    fp8_stream_kernel(const __grid_constant__ Fp8StreamParams p) {
   pdl_wait();  // the previous kernel of the stream has completed
   pdl_trigger();
+  constexpr int WARPS = fp8_stream_warps<OP>();
   constexpr int SETS = OP == FP8_STREAM_UP ? 2 : 1;
+  constexpr int AHEAD = 4 / SETS;  // k-blocks of a warp whose loads are in flight
   using T = typename std::conditional<OP == FP8_STREAM_DOWN, float, uint16_t>::type;
-  __shared__ float s_sum[kFp8StreamWarps][SETS][16][8];
+  extern __shared__ __align__(16) uint8_t s_codes[];
+  __shared__ float s_sum[WARPS][SETS][16][8];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int n0 = blockIdx.x * 16;
-  const int rows_n = OP == FP8_STREAM_UP ? p.N / 2 : p.N;  // output columns
+  const int cols = OP == FP8_STREAM_UP ? p.N / 2 : p.N;  // output columns
   const int k_blocks = (p.K + kFp8Block - 1) / kFp8Block, n_blocks = (p.N + kFp8Block - 1) / kFp8Block;
   const bool routed = p.top_k > 0;
-  int expert = 0, kb0 = warp, step = kFp8StreamWarps;
+  // this CTA's activation rows, and this warp's share: rows of one weight, from
+  // k-block kb0 on
+  int expert = 0, kb0 = warp, step = WARPS, row0 = 0, rows = p.rows;
   bool busy = true;
   float weight = 1.0f;
-  const T* xrow = nullptr;
-  if (!routed) {
-    if (g < p.rows) xrow = static_cast<const T*>(p.x) + (int64_t)g * p.ldx;
-  } else if (OP == FP8_STREAM_DOWN) {
-    // warps per slot, as many as fit
-    const int per = kFp8StreamWarps / p.top_k, slot = warp / per;
+  const T* x = static_cast<const T*>(p.x);
+  if (routed && OP == FP8_STREAM_DOWN) {
+    const int per = WARPS / p.top_k, slot = warp / per;  // warps per slot
+    rows = p.top_k;
+    x += (int64_t)blockIdx.y * p.top_k * p.ldx;
     busy = slot < p.top_k;
     if (busy) {
       const int64_t r = (int64_t)blockIdx.y * p.top_k + slot;
@@ -843,18 +801,69 @@ __global__ void __launch_bounds__(32 * kFp8StreamWarps) fp8_stream_kernel(const 
       weight = mul_rn(bf16_to_f32(p.gate[r]), p.scaling);
       kb0 = warp % per;
       step = per;
-      if (g == 0) xrow = static_cast<const T*>(p.x) + r * p.ldx;
+      row0 = slot;
     }
-  } else {
+  } else if (routed) {
+    rows = 1;
+    x += (int64_t)(blockIdx.y / p.top_k) * p.ldx;
     expert = checked_expert(p.top_idx[blockIdx.y], p.experts);
-    if (g == 0) xrow = static_cast<const T*>(p.x) + (int64_t)(blockIdx.y / p.top_k) * p.ldx;
   }
+  const int my_rows = routed ? 1 : rows;  // rows that share this warp's weight
+  const uint8_t* w = p.wq + ((int64_t)expert * p.N + n0 + g) * p.K + 16 * t;
+  const float* ws = p.ws + ((int64_t)expert * n_blocks + n0 / kFp8Block) * k_blocks;
+  const int64_t set_off = (int64_t)cols * p.K, ws_off = (int64_t)(cols / kFp8Block) * k_blocks;
+  uint4 a[AHEAD][SETS][2][2];  // [block][set][row g, g + 8][64-byte half]
+  float sw[AHEAD][SETS];
+  auto load = [&](int i, int kb) {
+    const bool in = busy && kb < k_blocks;
+#pragma unroll
+    for (int s = 0; s < SETS; ++s) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int col = kb * kFp8Block + 64 * j;
+          a[i][s][r][j] = make_uint4(0u, 0u, 0u, 0u);
+          if (in && col + 16 * t < p.K && n0 + g + 8 * r < cols)
+            a[i][s][r][j] = ldg_stream(reinterpret_cast<const uint4*>(w + s * set_off + (int64_t)8 * r * p.K + col));
+        }
+      sw[i][s] = in ? __ldg(ws + s * ws_off + kb) : 0.0f;
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i) load(i, kb0 + i * step);
+  const int pitch = fp8_stream_pitch(p.K);
+  float* scales = reinterpret_cast<float*>(s_codes + (size_t)rows * pitch);
+  fp8_stream_quantize<T, 32 * WARPS>(x, p.ldx, rows, p.K, s_codes, scales);
+  __syncthreads();
+  // rows past my_rows read row0's codes; their sums are not stored
+  const uint8_t* b_row = s_codes + (size_t)(row0 + (g < my_rows ? g : 0)) * pitch + 16 * t;
+  const float* sx0 = scales + (row0 + (2 * t < my_rows ? 2 * t : 0)) * k_blocks;
+  const float* sx1 = scales + (row0 + (2 * t + 1 < my_rows ? 2 * t + 1 : 0)) * k_blocks;
   float acc[SETS][4] = {};
-  if (busy) {
-    const uint8_t* w = p.wq + ((int64_t)expert * p.N + n0) * p.K;
-    const float* ws = p.ws + ((int64_t)expert * n_blocks + n0 / kFp8Block) * k_blocks;
-    fp8_stream_blocks<SETS, T>(xrow, w, (int64_t)rows_n * p.K, rows_n - n0, ws,
-                               (int64_t)(rows_n / kFp8Block) * k_blocks, p.K, kb0, step, acc);
+  for (int base = kb0; busy && base < k_blocks; base += AHEAD * step) {
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const int kb = base + i * step;
+      if (kb >= k_blocks) break;
+      const uint4 b0 = *reinterpret_cast<const uint4*>(b_row + kb * kFp8Block);
+      const uint4 b1 = *reinterpret_cast<const uint4*>(b_row + kb * kFp8Block + 64);
+      const float s0 = sx0[kb], s1 = sx1[kb];
+#pragma unroll
+      for (int s = 0; s < SETS; ++s) {
+        float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        mma_e4m3_16x8x32(d, a[i][s][0][0].x, a[i][s][1][0].x, a[i][s][0][0].y, a[i][s][1][0].y, b0.x, b0.y);
+        mma_e4m3_16x8x32(d, a[i][s][0][0].z, a[i][s][1][0].z, a[i][s][0][0].w, a[i][s][1][0].w, b0.z, b0.w);
+        mma_e4m3_16x8x32(d, a[i][s][0][1].x, a[i][s][1][1].x, a[i][s][0][1].y, a[i][s][1][1].y, b1.x, b1.y);
+        mma_e4m3_16x8x32(d, a[i][s][0][1].z, a[i][s][1][1].z, a[i][s][0][1].w, a[i][s][1][1].w, b1.z, b1.w);
+        const float f0 = s0 * sw[i][s], f1 = s1 * sw[i][s];
+        acc[s][0] = fmaf(d[0], f0, acc[s][0]);
+        acc[s][1] = fmaf(d[1], f1, acc[s][1]);
+        acc[s][2] = fmaf(d[2], f0, acc[s][2]);
+        acc[s][3] = fmaf(d[3], f1, acc[s][3]);
+      }
+      load(i, kb + AHEAD * step);
+    }
   }
 #pragma unroll
   for (int s = 0; s < SETS; ++s) {
@@ -866,24 +875,24 @@ __global__ void __launch_bounds__(32 * kFp8StreamWarps) fp8_stream_kernel(const 
   __syncthreads();
   if (threadIdx.x >= 128) return;
   const int n = threadIdx.x & 15, c = threadIdx.x >> 4;  // output column n0 + n of activation row c
-  if (c >= (routed ? 1 : p.rows) || n0 + n >= rows_n) return;
+  if (c >= my_rows || n0 + n >= cols) return;
   float sum[SETS];
 #pragma unroll
   for (int s = 0; s < SETS; ++s) {
     sum[s] = s_sum[0][s][n][c];
 #pragma unroll
-    for (int i = 1; i < kFp8StreamWarps; ++i) sum[s] += s_sum[i][s][n][c];
+    for (int i = 1; i < WARPS; ++i) sum[s] += s_sum[i][s][n][c];
   }
   const int64_t row = routed ? blockIdx.y : c;
   if constexpr (OP == FP8_STREAM_UP) {
     float g0 = sum[0], g1 = 0.0f;
     swiglu_pair_f32(g0, g1, sum[1], 0.0f);
-    p.hidden[row * rows_n + n0 + n] = g0;
+    p.hidden[row * cols + n0 + n] = g0;
   } else {
     uint16_t y = f32_to_bf16(sum[0]);
     if (OP == FP8_STREAM_DOWN && routed && p.shared != nullptr)
-      y = f32_to_bf16(add_rn(bf16_to_f32(y), bf16_to_f32(p.shared[row * rows_n + n0 + n])));
-    p.out[row * rows_n + n0 + n] = y;
+      y = f32_to_bf16(add_rn(bf16_to_f32(y), bf16_to_f32(p.shared[row * cols + n0 + n])));
+    p.out[row * cols + n0 + n] = y;
   }
 }
 
@@ -1042,19 +1051,36 @@ int run_fp8_gemm(const Fp8Gemm& g, cudaStream_t stream) {
   return pair ? fp8_launch<2, FP8_PLAIN>(p, units, stream) : fp8_launch<1, FP8_PLAIN>(p, units, stream);
 }
 
+constexpr size_t kFp8StreamSmemMax = 160 * 1024;
+
 template <int OP>
 static int fp8_stream_launch(const Fp8StreamParams& p, int groups, cudaStream_t stream) {
+  auto kernel = fp8_stream_kernel<OP>;
+  static DeviceOnce attr;
+  const int rc = device_once(attr, [&](int dev) {
+    const cudaError_t e =
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kFp8StreamSmemMax);
+    if (e != cudaSuccess)
+      return set_error(PRAXIS_B200_ECUDA, "fp8 stream smem attribute (device %d): %s", dev, cudaGetErrorString(e));
+    return (int)PRAXIS_B200_OK;
+  });
+  if (rc) return rc;
   const int cols = OP == FP8_STREAM_UP ? p.N / 2 : p.N;
-  launch_pdl(fp8_stream_kernel<OP>, dim3((unsigned)((cols + 15) / 16), (unsigned)groups), dim3(32 * kFp8StreamWarps), 0,
-             stream, p);
+  const int rows = p.top_k == 0 ? p.rows : OP == FP8_STREAM_DOWN ? p.top_k : 1;
+  launch_pdl(kernel, dim3((unsigned)((cols + 15) / 16), (unsigned)groups), dim3(32 * fp8_stream_warps<OP>()),
+             fp8_stream_smem(rows, p.K), stream, p);
   return check_launch("fp8_stream");
 }
 
 // Whether a product of `rows` rows goes through the streaming kernels: dense up
 // to the 8 rows that share a weight; routed slots read their expert's weight
-// each for itself, so as long as they are few.
-static bool fp8_streams(int64_t rows, int top_k, int experts) {
-  return top_k == 0 ? rows <= 8 : rows * top_k <= 16 || rows * top_k <= (experts < 64 ? experts : 64);
+// each for itself, so as long as they are few. The quantized rows have to fit
+// the shared memory (k_up: columns of the rows, k_down: of the hidden rows, 0
+// for a linear product).
+static bool fp8_streams(int64_t rows, int top_k, int experts, int k_up, int k_down) {
+  if (top_k == 0 ? rows > 8 : rows * top_k > 16 && rows * top_k > (experts < 64 ? experts : 64)) return false;
+  return fp8_stream_smem(top_k == 0 ? (int)rows : 1, k_up) <= kFp8StreamSmemMax &&
+         fp8_stream_smem(top_k == 0 ? (int)rows : top_k, k_down) <= kFp8StreamSmemMax;
 }
 
 static int run_fp8_stream_linear(const Fp8StreamParams& p, cudaStream_t stream) {

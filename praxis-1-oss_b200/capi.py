@@ -234,6 +234,8 @@ def library_path() -> Path:
 def load(build_if_missing: bool = False) -> C.CDLL:
     """Load (once) and return the library with typed entry points."""
     global _LIB
+    if _LIB is not None:
+        return _LIB
     with _LOCK:
         if _LIB is not None:
             return _LIB

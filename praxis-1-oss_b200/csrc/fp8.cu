@@ -696,7 +696,7 @@ struct Fp8StreamParams {
 // DOWN has two warps for each of up to 8 slots.
 template <int OP>
 __host__ __device__ constexpr int fp8_stream_warps() {
-  return OP == FP8_STREAM_DOWN ? 16 : 8;
+  return OP == FP8_STREAM_DOWN ? 16 : OP == FP8_STREAM_UP ? 4 : 8;
 }
 
 // Quantized activation rows in shared memory: row pitch (64 bytes more than a
@@ -769,7 +769,7 @@ __device__ __forceinline__ void mma_e4m3_16x8x32(float (&d)[4], uint32_t a0, uin
 // blockIdx.x: 16 weight rows (UP: 16 hidden columns); blockIdx.y: dense: 0;
 // UP: the routed slot; DOWN: the token.
 template <int OP>
-__global__ void __launch_bounds__(32 * fp8_stream_warps<OP>(), OP == FP8_STREAM_DOWN ? 1 : 2)
+__global__ void __launch_bounds__(32 * fp8_stream_warps<OP>(), 16 / fp8_stream_warps<OP>())
     fp8_stream_kernel(const __grid_constant__ Fp8StreamParams p) {
   pdl_wait();  // the previous kernel of the stream has completed
   pdl_trigger();

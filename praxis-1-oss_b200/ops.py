@@ -722,15 +722,24 @@ def moe_forward(x: Tensor, top_idx: Tensor | None, gate: Tensor | None, gate_up_
 
 
 # -- block-scaled FP8 weights ------------------------------------------------
-def _fp8_weight(q: Tensor, scale: Tensor, name: str, ndim: int) -> None:
-    """E4M3 values [.., N, K] with one fp32 scale per 128 x 128 block."""
+def _is(t: Tensor, dtype, ndim: int, device: int) -> bool:
+    """A contiguous CUDA tensor of this type, rank and device ordinal."""
+    return (isinstance(t, Tensor) and t.dtype is dtype and t.ndim == ndim and t.get_device() == device
+            and t.is_contiguous())
+
+
+def _fp8_weight(q: Tensor, scale: Tensor, name: str, ndim: int) -> int:
+    """E4M3 values [.., N, K] with one fp32 scale per 128 x 128 block; returns
+    their device ordinal."""
     _need(q, name + "_q", F8, ndim)
-    _need(scale, name + "_scale", torch.float32, ndim)
-    _same_device(q, scale)
+    device = q.get_device()
+    if not _is(scale, torch.float32, ndim, device):
+        _need(scale, name + "_scale", torch.float32, ndim, q.device)
     shape = q.shape
     if shape[:-2] + (-(-shape[-2] // 128), -(-shape[-1] // 128)) != scale.shape:
         raise ValueError(f"{name}_scale: got {tuple(scale.shape)}, expected one scale per 128 x 128 block of "
                          f"{tuple(shape)}")
+    return device
 
 
 def _fp8_rows(x: Tensor, width: int) -> tuple[Tensor, int, int]:
@@ -752,16 +761,16 @@ def _fp8_rows(x: Tensor, width: int) -> tuple[Tensor, int, int]:
     return x, rows, pitch
 
 
-def _same_device(x: Tensor, *others) -> None:
-    device = x.get_device()
-    for t in others:
-        if t is not None and t.get_device() != device:
-            raise ValueError("tensors must share a device")
+def _on(t: Tensor, device: int) -> None:
+    if t.get_device() != device:
+        raise ValueError("tensors must share a device")
 
 
 def _inference_only(*tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError("the FP8 products support inference only")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError("the FP8 products support inference only")
 
 
 def fp8_quantize(x: Tensor) -> tuple[Tensor, Tensor]:
@@ -805,32 +814,33 @@ def fp8_linear(x: Tensor, w_q: Tensor, w_scale: Tensor) -> Tensor:
     x [.., K] bf16 (2-D rows may be a column slice of a wider tensor) is
     quantized in the call as by :func:`fp8_quantize`; the products are summed
     in fp32. K % 16 == 0, any N, any number of rows. Inference only."""
-    _fp8_weight(w_q, w_scale, "w", 2)
+    device = _fp8_weight(w_q, w_scale, "w", 2)
     n, k = w_q.shape
     x, r, pitch = _fp8_rows(x, k)
-    _same_device(x, w_q)
+    _on(x, device)
     _inference_only(x)
     out = x.new_empty(x.shape[:-1] + (n,))
     lib = capi.load()
     size = lib.praxis_b200_fp8_linear_workspace_size(r, n, k)
-    ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
-    device, stream = _place(x)
+    ws = w_q.new_empty((size,), dtype=torch.uint8) if size else None
+    stream = torch._C._cuda_getCurrentRawStream(device)
     _run(device, lib.praxis_b200_fp8_linear, x.data_ptr(), r, k, pitch, w_q.data_ptr(), w_scale.data_ptr(), n,
          out.data_ptr(), None if ws is None else ws.data_ptr(), size, device, stream)
     return out
 
 
 def _fp8_ffn_shapes(gate_up_q: Tensor, gate_up_scale: Tensor, down_q: Tensor, down_scale: Tensor, ndim: int
-                    ) -> tuple[int, int, int]:
-    """(E, C, F) of a gate/up and a down weight that belong together."""
-    _fp8_weight(gate_up_q, gate_up_scale, "gate_up", ndim)
-    _fp8_weight(down_q, down_scale, "down", ndim)
-    _same_device(gate_up_q, down_q)
-    f2, c = gate_up_q.shape[-2:]
+                    ) -> tuple[int, int, int, int]:
+    """(E, C, F, device ordinal) of a gate/up and a down weight that belong together."""
+    device = _fp8_weight(gate_up_q, gate_up_scale, "gate_up", ndim)
+    if _fp8_weight(down_q, down_scale, "down", ndim) != device:
+        raise ValueError("tensors must share a device")
+    shape = gate_up_q.shape
+    f2, c = shape[-2:]
     f = f2 // 2
-    if f2 % 2 or c % 128 or f % 128 or not c or not f or down_q.shape != gate_up_q.shape[:-2] + (c, f):
+    if f2 % 2 or c % 128 or f % 128 or not c or not f or down_q.shape != shape[:-2] + (c, f):
         raise ValueError("expected gate_up_q [.., 2F, C] and down_q [.., C, F], C and F multiples of 128")
-    return (gate_up_q.shape[0] if ndim == 3 else 1), c, f
+    return (shape[0] if ndim == 3 else 1), c, f, device
 
 
 def _ptr(t: Tensor | None):
@@ -839,13 +849,13 @@ def _ptr(t: Tensor | None):
 
 def _fp8_ffn(x: Tensor, t: int, top_idx: Tensor | None, gate: Tensor | None, shared: Tensor | None, out: Tensor | None,
              weights: tuple, sizes: tuple, scaling: float, tail=None) -> None:
-    e, c, f = sizes
+    e, c, f, device = sizes
     k = 0 if top_idx is None else top_idx.shape[1]
     lib = capi.load()
     size = lib.praxis_b200_fp8_ffn_workspace_size(t, k, e, c, f)
-    ws = torch.empty(size, dtype=torch.uint8, device=x.device)
     gate_up_q, gate_up_scale, down_q, down_scale = weights
-    device, stream = _place(x)
+    ws = gate_up_q.new_empty((size,), dtype=torch.uint8)
+    stream = torch._C._cuda_getCurrentRawStream(device)
     args = capi.Fp8FfnArgs(  # in the order of the struct
         x.data_ptr(), _ptr(top_idx), _ptr(gate), _ptr(shared), _ptr(out), gate_up_q.data_ptr(),
         gate_up_scale.data_ptr(), down_q.data_ptr(), down_scale.data_ptr(), t, c, f, e, k, scaling, ws.data_ptr(),
@@ -864,7 +874,7 @@ def fp8_mlp(x: Tensor, gate_up_q: Tensor, gate_up_scale: Tensor, down_q: Tensor,
     x, t, pitch = _fp8_rows(x, sizes[1])
     if pitch != sizes[1]:
         raise ValueError("x: expected a contiguous CUDA bf16 tensor")
-    _same_device(x, gate_up_q)
+    _on(x, sizes[3])
     _inference_only(x)
     if out is None:
         out = torch.empty_like(x)
@@ -886,20 +896,21 @@ def fp8_moe_forward(x: Tensor, top_idx: Tensor, gate: Tensor, gate_up_q: Tensor,
     weighted combine (+ ``shared``). With ``tail`` the result is ``(new
     residual, normed rows or None)`` as there. Inference only."""
     sizes = _fp8_ffn_shapes(gate_up_q, gate_up_scale, down_q, down_scale, 3)
-    e, c, _ = sizes
-    _need(x, "x", BF16, 2)
+    e, c, _, device = sizes
+    if not (_is(x, BF16, 2, device) and _is(top_idx, torch.int64, 2, device) and _is(gate, BF16, 2, device)
+            and (shared is None or _is(shared, BF16, 2, device))):
+        for ten, name, dtype in ((x, "x", BF16), (top_idx, "top_idx", torch.int64), (gate, "gate", BF16),
+                                 (shared, "shared", BF16)):
+            if ten is not None or name != "shared":
+                _need(ten, name, dtype, 2, gate_up_q.device)
     t = x.shape[0]
     if x.shape[1] != c:
         raise ValueError(f"x: expected {c} columns, got {x.shape[1]}")
-    _need(top_idx, "top_idx", torch.int64, 2)
-    _need(gate, "gate", BF16, 2)
-    if top_idx.shape[0] != t or gate.shape != top_idx.shape or not 1 <= top_idx.shape[1] <= min(8, e):
+    shape = top_idx.shape
+    if shape[0] != t or gate.shape != shape or not 1 <= shape[1] <= min(8, e):
         raise ValueError("top_idx / gate: expected [T, k], 1 <= k <= min(8, E)")
-    if shared is not None:
-        _need(shared, "shared", BF16, 2)
-        if shared.shape != x.shape:
-            raise ValueError("shared must have the shape of x")
-    _same_device(x, gate_up_q, top_idx, gate, shared)
+    if shared is not None and shared.shape != x.shape:
+        raise ValueError("shared must have the shape of x")
     _inference_only(x, gate, shared)
     weights = (gate_up_q, gate_up_scale, down_q, down_scale)
     if tail is not None:

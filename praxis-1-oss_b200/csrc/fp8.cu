@@ -567,7 +567,7 @@ __device__ __forceinline__ void fp8_gemm_body(const Fp8GemmParams& p) {
       }
       const int n_out = n;
       const int64_t row_out = row;
-      const bool store = row_in_tile < valid;
+      const int valid_out = valid;
       if (u + step < total) fetch(u + step);
       if constexpr (MODE == FP8_SWIGLU) {
         // 64 hidden columns 128 n_out + 64 h ..; the other half's warps hold the
@@ -582,7 +582,7 @@ __device__ __forceinline__ void fp8_gemm_body(const Fp8GemmParams& p) {
         mx[h * 128] = a;
         named_sync(kFp8BarMax, 32 * S::EPI_WARPS);
         a = fmaxf(a, mx[(h ^ 1) * 128]);
-        if (store) {
+        if (row_in_tile < valid_out) {
           const float r = div_rn(kE4m3Max, a);
           uint8_t* dst = p.hq + row_out * F + n_out * 128 + 64 * h;
 #pragma unroll
@@ -600,35 +600,45 @@ __device__ __forceinline__ void fp8_gemm_body(const Fp8GemmParams& p) {
         }
       } else {
         const int col0 = n_out * 256 + 128 * h;
-        if (p.tma_out) {
-          // two boxes of 32 rows x 64 columns in the TMA 128-byte swizzle; of a
-          // table's tile the padding rows are written too (scratch), never
-          // rows of the next tile
-          uint8_t* box = sOut + (warp - S::EPI_WARP0) * S::OUT_BOX;
+        // two boxes of 32 rows x 64 columns in the TMA 128-byte swizzle
+        uint8_t* box = sOut + (warp - S::EPI_WARP0) * S::OUT_BOX;
+        const int box_rows = valid_out - 128 * (int)rank - 32 * (int)quad;  // rows of the box that exist
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            if (lane == 0) bulk_wait_group_read0();
-            __syncwarp();
+        for (int i = 0; i < 2; ++i) {
+          const int col = col0 + 64 * i;
+          if (p.tma_out && lane == 0) bulk_wait_group_read0();
+          __syncwarp();
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {
-              const float* v = acc + 64 * i + 8 * c;
-              *reinterpret_cast<uint4*>(box + lane * 128 + ((c ^ (lane & 7)) << 4)) =
-                  make_uint4(cvt_bf16x2(v[0], v[1]), cvt_bf16x2(v[2], v[3]), cvt_bf16x2(v[4], v[5]),
-                             cvt_bf16x2(v[6], v[7]));
-            }
+          for (int c = 0; c < 8; ++c) {
+            const float* v = acc + 64 * i + 8 * c;
+            *reinterpret_cast<uint4*>(box + lane * 128 + ((c ^ (lane & 7)) << 4)) =
+                make_uint4(cvt_bf16x2(v[0], v[1]), cvt_bf16x2(v[2], v[3]), cvt_bf16x2(v[4], v[5]),
+                           cvt_bf16x2(v[6], v[7]));
+          }
+          if (p.tma_out) {
+            // of a table's tile the padding rows are written too (scratch),
+            // never rows of the next tile
             fence_proxy_async_shared();
             __syncwarp();
-            if (lane == 0 && store && col0 + 64 * i < p.N) {  // row 0 of the box has a routed row
-              tma_store_2d(&p.tmap_out, box, col0 + 64 * i, (int32_t)row_out);
+            if (lane == 0 && box_rows > 0 && col < p.N) {
+              tma_store_2d(&p.tmap_out, box, col, (int32_t)row_out);
               bulk_commit_group();
             }
-          }
-        } else if (store) {
-          // rows of N bf16 that are not multiples of 16 bytes
-          uint16_t* dst = p.out + row_out * p.N + col0;
+          } else {
+            // rows that are no multiple of 16 bytes: a lane writes column lane
+            // and lane + 32 of each row
+            __syncwarp();
+            const int64_t r0 = row_out - (int64_t)lane;
+            for (int r = 0; r < min(box_rows, 32); ++r) {
+              uint16_t* dst = p.out + (r0 + r) * p.N + col;
 #pragma unroll
-          for (int j = 0; j < 128; ++j)
-            if (col0 + j < p.N) dst[j] = f32_to_bf16(acc[j]);
+              for (int j = 0; j < 2; ++j) {
+                const int c = (int)lane + 32 * j;
+                if (col + c < p.N)
+                  dst[c] = *reinterpret_cast<const uint16_t*>(box + r * 128 + (((c >> 3) ^ (r & 7)) << 4) + (c & 7) * 2);
+              }
+            }
+          }
         }
       }
       __syncwarp();

@@ -427,7 +427,7 @@ template <int P>
 __global__ void __launch_bounds__(256) route_groups_kernel(const float* __restrict__ logits,
                                                            const float* __restrict__ bias, int64_t tokens, int experts,
                                                            int top_k, int activation, int groups, int top_groups,
-                                                           int top2, int lpg_log2, int64_t* __restrict__ top_idx,
+                                                           int top2, int lpg_log2, int wide, int64_t* __restrict__ top_idx,
                                                            uint16_t* __restrict__ gate) {
   pdl_wait();  // the previous kernel of the stream has completed
   pdl_trigger();
@@ -445,10 +445,24 @@ __global__ void __launch_bounds__(256) route_groups_kernel(const float* __restri
   float score[P];
   float lmax = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < P; ++i) {
-    score[i] = i < mine ? lr[i] : -INFINITY;
-    lmax = fmaxf(lmax, score[i]);
+  for (int i = 0; i < P; ++i) score[i] = -INFINITY;
+  if (wide) {  // 16-byte loads: every lane's share starts on a multiple of 4 and is one
+#pragma unroll
+    for (int i = 0; i < P; i += 4)
+      if (i < mine) {
+        const float4 v = __ldg(reinterpret_cast<const float4*>(lr + i));
+        score[i] = v.x;
+        score[i + 1] = v.y;
+        score[i + 2] = v.z;
+        score[i + 3] = v.w;
+      }
+  } else {
+#pragma unroll
+    for (int i = 0; i < P; ++i)
+      if (i < mine) score[i] = lr[i];
   }
+#pragma unroll
+  for (int i = 0; i < P; ++i) lmax = fmaxf(lmax, score[i]);
   if (activation == PRAXIS_B200_SOFTMAX) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) lmax = fmaxf(lmax, __shfl_xor_sync(kAll, lmax, o));
@@ -467,7 +481,7 @@ __global__ void __launch_bounds__(256) route_groups_kernel(const float* __restri
     for (int i = 0; i < P; ++i) score[i] = div_rn(score[i], total);
   } else {
 #pragma unroll
-    for (int i = 0; i < P; ++i) score[i] = div_rn(1.0f, add_rn(1.0f, expf(-score[i])));
+    for (int i = 0; i < P; ++i) score[i] = __frcp_rn(add_rn(1.0f, expf(-score[i])));
   }
   // order-preserving keys of the biased scores; 0 (below every number) marks
   // no expert, a closed group or a pick already made
@@ -639,9 +653,10 @@ int run_route_groups(const float* logits, const float* bias, int64_t tokens, int
   const int per = (experts / groups + (1 << lpg_log2) - 1) >> lpg_log2;
   const dim3 grid((unsigned)((tokens + 7) / 8));
   const int top2 = group_score == PRAXIS_B200_GROUP_TOP2;
+  const int wide = per % 4 == 0 && (experts / groups) % 4 == 0 && ((uintptr_t)logits & 15) == 0;
 #define PRAXIS_ROUTE_GROUPS(P)                                                                                     \
   launch_pdl(route_groups_kernel<P>, grid, dim3(256), 0, stream, logits, bias, tokens, experts, top_k, activation, \
-             groups, top_groups, top2, lpg_log2, top_idx, gate)
+             groups, top_groups, top2, lpg_log2, wide, top_idx, gate)
   // experts per lane: 2^ceil(log2 groups) lanes' shares, at most 16 (256
   // experts in 9 or 17 groups leave almost half of the lanes without one)
   if (per <= 4) PRAXIS_ROUTE_GROUPS(4);

@@ -199,25 +199,31 @@ struct Fp8GemmParams {
 // Named barriers (the last two kinds one per tensor-memory buffer).
 constexpr uint32_t kFp8BarMax = 1;   // SwiGLU row maxima: the epilogue warps
 constexpr uint32_t kFp8BarSums = 2;  // a buffer holds its block sums: relay -> epilogue
-constexpr uint32_t kFp8BarGo = 4;    // a buffer is read and its next operands are there: epilogue, relay -> issuer
+constexpr uint32_t kFp8BarGo = 6;    // a buffer is read and its next operands are there: epilogue, relay -> issuer
 
-template <int CTAS>
+template <int CTAS, int BN>
 struct Fp8Shape {
   static constexpr int A_BYTES = 128 * 128;
-  static constexpr int B_BYTES = 256 / CTAS * 128;
+  static constexpr int B_BYTES = BN / CTAS * 128;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr int STAGES = CTAS == 2 ? 6 : 4;
-  static constexpr int OUT_BOX = 4096;  // 32 rows x 64 bf16 per epilogue warp
-  static constexpr int EPI_WARPS = 8;
+  static constexpr int STAGES = BN == 64 ? 8 : CTAS == 2 ? 6 : 4;
+  static constexpr int BUFS = BN == 64 ? 4 : 2;  // tensor-memory buffers of BN columns
+  static constexpr int OUT_BOX = 4096;           // 32 rows x 64 bf16 per epilogue warp
+  static constexpr int EPI_WARPS = BN == 64 ? 4 : 8;
+  static constexpr int COLS = 4 * BN / EPI_WARPS;  // columns per epilogue thread
   // Registers: 12 warps launch with 168 each (64512 in all); the first four
   // give some back, and the epilogue's 128 sums and two 16-column loads in
-  // flight fit without spilling.
+  // flight fit without spilling. 8 warps (BN = 64) have enough as they are.
   static constexpr int EPI_WARP0 = 4;
   static constexpr int THREADS = 32 * (EPI_WARP0 + EPI_WARPS);
+  static constexpr bool SPLIT_REGS = EPI_WARPS == 8;
   static constexpr int LAUNCH_REGS = 168, FRONT_REGS = 40, EPI_REGS = 232;
-  static_assert(32 * EPI_WARP0 * FRONT_REGS + 32 * EPI_WARPS * EPI_REGS <= THREADS * LAUNCH_REGS, "register split");
+  static_assert(!SPLIT_REGS ||
+                    32 * EPI_WARP0 * FRONT_REGS + 32 * EPI_WARPS * EPI_REGS <= THREADS * LAUNCH_REGS,
+                "register split");
   static constexpr size_t SMEM_BYTES = 1024 + (size_t)STAGES * STAGE_BYTES + EPI_WARPS * OUT_BOX + 256;
   static_assert(SMEM_BYTES <= 232448, "shared memory budget");
+  static_assert(8 * (2 * STAGES + 3) <= 256 && BUFS <= 4, "barriers");
 };
 
 // E4M3 x E4M3 -> F32 (kind::f8f6f4), K-major operands, K = 32 per MMA.
@@ -334,11 +340,12 @@ __device__ constexpr uint32_t chunk_col(int c) {
   return 16 * c + (MODE == FP8_SWIGLU && c >= 4 ? 64 : 0);
 }
 
-template <int CTAS, int MODE>
+template <int CTAS, int BN, int MODE>
 __device__ __forceinline__ void fp8_gemm_body(const Fp8GemmParams& p) {
   pdl_wait();  // the previous kernel of the stream has completed
   pdl_trigger();
-  using S = Fp8Shape<CTAS>;
+  using S = Fp8Shape<CTAS, BN>;
+  static_assert(MODE == FP8_PLAIN || BN == 256, "a SwiGLU tile is one block of 128 hidden columns");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sA = smem;
@@ -368,7 +375,7 @@ __device__ __forceinline__ void fp8_gemm_body(const Fp8GemmParams& p) {
   }
   if (warp == 1) {
     if constexpr (CTAS == 1) {
-      tmem_alloc(tmem_slot, 512);
+      tmem_alloc(tmem_slot, S::BUFS * BN);
       tmem_relinquish();
     } else {
       tmem_alloc_pair(tmem_slot, 512);
@@ -383,7 +390,7 @@ __device__ __forceinline__ void fp8_gemm_body(const Fp8GemmParams& p) {
   const uint32_t tmem = *tmem_slot;
 
   const int F = p.N / 2;
-  const int n_tiles = MODE == FP8_SWIGLU ? F / 128 : (p.N + 255) / 256;
+  const int n_tiles = MODE == FP8_SWIGLU ? F / 128 : (p.N + BN - 1) / BN;
   const int num_m =
       p.tiles != nullptr ? p.num_tiles[CTAS - 1] : (int)((p.rows + CTAS * kTileRows - 1) / (CTAS * kTileRows));
   const int total = num_m * n_tiles;
@@ -395,12 +402,12 @@ __device__ __forceinline__ void fp8_gemm_body(const Fp8GemmParams& p) {
   const int turns = first < total ? ((total - 1 - first) / step + 1) * k_blocks : 0;
 
   if (warp < S::EPI_WARP0) {
-    regs_down<S::FRONT_REGS>();
+    if constexpr (S::SPLIT_REGS) regs_down<S::FRONT_REGS>();
     if (warp == 0) {
       // ---------------- TMA producer (every CTA) ----------------
-      // one lane per copy: A, the first 128 weight rows, the next 128 (CTAS = 1)
+      // one lane per copy: A, the weight rows, of 256 in two copies (CTAS = 1)
       const uint32_t full_leader = CTAS == 1 ? 0u : mapa_shared(smem_u32(full), 0);
-      constexpr uint32_t kCopies = CTAS == 1 ? 3 : 2;
+      constexpr uint32_t kCopies = CTAS == 1 && BN == 256 ? 3 : 2;
       const CUtensorMap* map = lane == 0 ? &p.tmap_a : &p.tmap_b;
       uint8_t* const dst0 = lane == 0 ? sA : sB + (lane == 2 ? 16384 : 0);
       const uint32_t dst_step = lane == 0 ? S::A_BYTES : S::B_BYTES;
@@ -412,7 +419,7 @@ __device__ __forceinline__ void fp8_gemm_body(const Fp8GemmParams& p) {
         // weight rows of columns 0..127 and 128..255 (of the leader and its peer)
         const int part = CTAS == 1 ? (lane == 2 ? 1 : 0) : (int)rank;
         const int row = lane == 0 ? t.row0 + 128 * (int)rank
-                                  : t.expert * p.N + (MODE == FP8_SWIGLU ? n * 128 + part * F : n * 256 + part * 128);
+                                  : t.expert * p.N + (MODE == FP8_SWIGLU ? n * 128 + part * F : n * BN + part * 128);
         for (int kb = 0; kb < k_blocks; ++kb) {
           ok = fp8_wait(&done[stage], phase ^ 1u, kErrTimeoutProducer);
           ok = __all_sync(0xffffffffu, ok);
@@ -432,17 +439,17 @@ __device__ __forceinline__ void fp8_gemm_body(const Fp8GemmParams& p) {
       }
     } else if (warp == 1 && rank == 0) {
       // ---------------- MMA issuer (leader) ----------------
-      constexpr uint32_t idesc = idesc_e4m3(128 * CTAS, 256);
+      constexpr uint32_t idesc = idesc_e4m3(128 * CTAS, BN);
       const uint64_t a_desc = smem_desc(smem_u32(sA), 16, 1024, kLayoutSwizzle128B);
       const uint32_t desc_hi = (uint32_t)(a_desc >> 32), a_lo = (uint32_t)a_desc;
       const uint32_t b_lo = (uint32_t)smem_desc(smem_u32(sB), 16, 1024, kLayoutSwizzle128B);
       uint32_t stage = 0, buf = 0;
-      for (int i = 0; i < turns; ++i, buf ^= 1u) {
-        named_sync(kFp8BarGo + buf, i < 2 ? 64 : 32 * (S::EPI_WARPS + 2));
+      for (int i = 0; i < turns; ++i) {
+        named_sync(kFp8BarGo + buf, i < S::BUFS ? 64 : 32 * (S::EPI_WARPS + 2));
         tc_fence_after();
         if (lane == 0) {
           const uint32_t a = a_lo + stage * (S::A_BYTES >> 4), b = b_lo + stage * (S::B_BYTES >> 4);
-          const uint32_t d = tmem + buf * 256;
+          const uint32_t d = tmem + buf * BN;
           tc_mma_e4m3<CTAS, 0>(d, a, b, desc_hi, idesc);
           tc_mma_e4m3<CTAS, 1>(d, a + 2, b + 2, desc_hi, idesc);
           tc_mma_e4m3<CTAS, 1>(d, a + 4, b + 4, desc_hi, idesc);
@@ -451,17 +458,18 @@ __device__ __forceinline__ void fp8_gemm_body(const Fp8GemmParams& p) {
         }
         __syncwarp();
         if (++stage == S::STAGES) stage = 0;
+        if (++buf == S::BUFS) buf = 0;
       }
-      // the epilogue's releases of the last two buffers
-      for (int i = turns < 2 ? 0 : turns - 2; i < turns; ++i)
-        named_sync(kFp8BarGo + (i & 1), 32 * (S::EPI_WARPS + 2));
+      // the epilogue's releases of the last buffers
+      for (int i = turns < S::BUFS ? 0 : turns - S::BUFS; i < turns; ++i)
+        named_sync(kFp8BarGo + i % S::BUFS, 32 * (S::EPI_WARPS + 2));
     } else if (warp == 2) {
       // ---------------- relay: products complete -> epilogue (every CTA) ----------------
       uint32_t stage = 0, phase = 0;
       for (int i = 0; i < turns; ++i) {
         fp8_wait(&done[stage], phase, kErrTimeoutEpilogue, 2000000000ull, false);
         __syncwarp();
-        named_sync(kFp8BarSums + (i & 1), 32 * (S::EPI_WARPS + 1));
+        named_sync(kFp8BarSums + i % S::BUFS, 32 * (S::EPI_WARPS + 1));
         if (++stage == S::STAGES) {
           stage = 0;
           phase ^= 1u;
@@ -474,27 +482,29 @@ __device__ __forceinline__ void fp8_gemm_body(const Fp8GemmParams& p) {
       bool ok = true;
       for (int i = 0; i < turns; ++i) {
         ok = ok && fp8_wait(&full[stage], stage_phase, kErrTimeoutMma);
-        if (CTAS == 2 && i >= 2) fp8_wait(&peer_free[buf], phase ^ 1u, kErrTimeoutMma, 2000000000ull, false);
+        if (CTAS == 2 && i >= S::BUFS) fp8_wait(&peer_free[buf], phase ^ 1u, kErrTimeoutMma, 2000000000ull, false);
         __syncwarp();
-        named_sync(kFp8BarGo + buf, i < 2 ? 64 : 32 * (S::EPI_WARPS + 2));
+        named_sync(kFp8BarGo + buf, i < S::BUFS ? 64 : 32 * (S::EPI_WARPS + 2));
         if (++stage == S::STAGES) {
           stage = 0;
           stage_phase ^= 1u;
         }
-        phase ^= buf;
-        buf ^= 1u;
+        if (++buf == S::BUFS) {
+          buf = 0;
+          phase ^= 1u;
+        }
       }
-      for (int i = turns < 2 ? 0 : turns - 2; i < turns; ++i)
-        named_sync(kFp8BarGo + (i & 1), 32 * (S::EPI_WARPS + 2));
+      for (int i = turns < S::BUFS ? 0 : turns - S::BUFS; i < turns; ++i)
+        named_sync(kFp8BarGo + i % S::BUFS, 32 * (S::EPI_WARPS + 2));
     }
   } else {
-    regs_up<S::EPI_REGS>();
+    if constexpr (S::SPLIT_REGS) regs_up<S::EPI_REGS>();
     // ---------------- epilogue (warps 4..19, every CTA) ----------------
     const uint32_t quad = (uint32_t)(warp & 3);
-    const int h = (warp - S::EPI_WARP0) >> 2;  // columns 128 h .. (SwiGLU: gate 64 h .. and up 128 + 64 h ..)
+    const int h = (warp - S::EPI_WARP0) >> 2;  // columns COLS h .. (SwiGLU: gate 64 h .. and up 128 + 64 h ..)
     const int row_in_cta = (int)(quad * 32 + lane);
     const uint32_t peer_free_leader = CTAS == 1 ? 0u : mapa_shared(smem_u32(peer_free), 0);
-    const uint32_t taddr = tmem + ((quad * 32u) << 16) + (MODE == FP8_SWIGLU ? 64u : 128u) * h;
+    const uint32_t taddr = tmem + ((quad * 32u) << 16) + (MODE == FP8_SWIGLU ? 64u : (uint32_t)S::COLS) * h;
     const int n_blocks = (p.N + kFp8Block - 1) / kFp8Block;
     // A unit's rows, columns and scale addresses, and the scales of its first
     // two k-blocks, are fetched while the previous unit is written out.
@@ -513,7 +523,7 @@ __device__ __forceinline__ void fp8_gemm_body(const Fp8GemmParams& p) {
       xs = p.xs + min(row, p.rows - 1);
       // the weight scales of this thread's columns: one row of blocks, or the
       // gate's and the up's
-      const int nb0 = MODE == FP8_SWIGLU ? n : min(2 * n + h, n_blocks - 1);
+      const int nb0 = MODE == FP8_SWIGLU ? n : min((n * BN + h * S::COLS) / kFp8Block, n_blocks - 1);
       ws = p.ws + ((int64_t)t.expert * n_blocks + nb0) * k_blocks;
       x0 = __ldg(xs);
       w00 = __ldg(ws);
@@ -527,12 +537,12 @@ __device__ __forceinline__ void fp8_gemm_body(const Fp8GemmParams& p) {
     uint32_t buf = 0, unit = 0;
     if (first < total) fetch(first);
     for (int u = first; u < total; u += step, ++unit) {
-      float acc[128];
+      float acc[S::COLS];
 #pragma unroll
-      for (int j = 0; j < 128; ++j) acc[j] = 0.0f;
+      for (int j = 0; j < S::COLS; ++j) acc[j] = 0.0f;
       uint32_t ra[16], rb[16];
-      for (int kb = 0; kb < k_blocks; ++kb, buf ^= 1u) {
-        const uint32_t tb = taddr + buf * 256;
+      for (int kb = 0; kb < k_blocks; ++kb) {
+        const uint32_t tb = taddr + buf * BN;
         const float f0 = x0 * w00, f1 = MODE == FP8_SWIGLU ? x0 * w01 : f0;
         x0 = x1;
         w00 = w10;
@@ -546,11 +556,11 @@ __device__ __forceinline__ void fp8_gemm_body(const Fp8GemmParams& p) {
         tc_fence_after();
         tc_ld_32x32b_x16(tb, ra);
 #pragma unroll
-        for (int c = 0; c < 8; c += 2) {
+        for (int c = 0; c < S::COLS / 16; c += 2) {
           tc_wait_ld();
           tc_ld_32x32b_x16(tb + chunk_col<MODE>(c + 1), rb);
           fp8_add_block(acc + 16 * c, ra, c < 4 ? f0 : f1);
-          if (c == 6) break;
+          if (c + 2 == S::COLS / 16) break;
           tc_wait_ld();
           tc_ld_32x32b_x16(tb + chunk_col<MODE>(c + 2), ra);
           fp8_add_block(acc + 16 * (c + 1), rb, c < 4 ? f0 : f1);
@@ -563,7 +573,8 @@ __device__ __forceinline__ void fp8_gemm_body(const Fp8GemmParams& p) {
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster(peer_free_leader + buf * 8);
         }
-        fp8_add_block(acc + 112, rb, f1);
+        fp8_add_block(acc + S::COLS - 16, rb, f1);
+        if (++buf == S::BUFS) buf = 0;
       }
       const int n_out = n;
       const int64_t row_out = row;
@@ -599,12 +610,12 @@ __device__ __forceinline__ void fp8_gemm_body(const Fp8GemmParams& p) {
           if (h == 0) p.hs[(int64_t)n_out * p.hs_ld + row_out] = div_rn(a, kE4m3Max);
         }
       } else {
-        const int col0 = n_out * 256 + 128 * h;
-        // two boxes of 32 rows x 64 columns in the TMA 128-byte swizzle
+        const int col0 = n_out * BN + S::COLS * h;
+        // boxes of 32 rows x 64 columns in the TMA 128-byte swizzle
         uint8_t* box = sOut + (warp - S::EPI_WARP0) * S::OUT_BOX;
         const int box_rows = valid_out - 128 * (int)rank - 32 * (int)quad;  // rows of the box that exist
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < S::COLS / 64; ++i) {
           const int col = col0 + 64 * i;
           if (p.tma_out && lane == 0) bulk_wait_group_read0();
           __syncwarp();
@@ -652,20 +663,21 @@ __device__ __forceinline__ void fp8_gemm_body(const Fp8GemmParams& p) {
   else cluster_sync();  // all tensor-memory reads and cross-CTA signals of the pair done
   if (warp == 1) {
     tc_fence_after();
-    if constexpr (CTAS == 1) tmem_dealloc(tmem, 512);
+    if constexpr (CTAS == 1) tmem_dealloc(tmem, S::BUFS * BN);
     else tmem_dealloc_pair(tmem, 512);
   }
 }
 
-template <int MODE>
-__global__ void __launch_bounds__(Fp8Shape<1>::THREADS, 1) fp8_gemm_kernel(const __grid_constant__ Fp8GemmParams p) {
-  fp8_gemm_body<1, MODE>(p);
+template <int BN, int MODE>
+__global__ void __launch_bounds__(Fp8Shape<1, BN>::THREADS, 1)
+    fp8_gemm_kernel(const __grid_constant__ Fp8GemmParams p) {
+  fp8_gemm_body<1, BN, MODE>(p);
 }
 
 template <int MODE>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Fp8Shape<2>::THREADS, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Fp8Shape<2, 256>::THREADS, 1)
     fp8_gemm_pair_kernel(const __grid_constant__ Fp8GemmParams p) {
-  fp8_gemm_body<2, MODE>(p);
+  fp8_gemm_body<2, 256, MODE>(p);
 }
 
 // ---------------------------------------------------------------------------
@@ -939,11 +951,11 @@ static int fp8_map(CUtensorMap* map, CUtensorMapDataType type, int elem, const v
 }
 
 // Launches on at most one CTA (pair) per SM; `units` bounds the work.
-template <int CTAS, int MODE>
+template <int CTAS, int BN, int MODE>
 static int fp8_launch(const Fp8GemmParams& p, int64_t units, cudaStream_t stream) {
-  using S = Fp8Shape<CTAS>;
+  using S = Fp8Shape<CTAS, BN>;
   auto kernel = [] {
-    if constexpr (CTAS == 1) return fp8_gemm_kernel<MODE>;
+    if constexpr (CTAS == 1) return fp8_gemm_kernel<BN, MODE>;
     else return fp8_gemm_pair_kernel<MODE>;
   }();
   static DeviceOnce attr;
@@ -955,7 +967,7 @@ static int fp8_launch(const Fp8GemmParams& p, int64_t units, cudaStream_t stream
     // setmaxnreg waits for registers that the launch does not have
     cudaFuncAttributes fa;
     e = cudaFuncGetAttributes(&fa, kernel);
-    if (e != cudaSuccess || fa.numRegs < S::LAUNCH_REGS)
+    if (e != cudaSuccess || (S::SPLIT_REGS && fa.numRegs < S::LAUNCH_REGS))
       return set_error(PRAXIS_B200_ECUDA, "fp8 gemm: built with %d registers a thread, needs %d", fa.numRegs,
                        S::LAUNCH_REGS);
     int n = sm_count();
@@ -1027,13 +1039,20 @@ struct Fp8Gemm {
 
 int run_fp8_gemm(const Fp8Gemm& g, cudaStream_t stream) {
   if (g.rows == 0) return PRAXIS_B200_OK;
+  const bool swiglu = g.out == nullptr;
+  const int64_t n_tiles = swiglu ? g.n / 256 : (g.n + 255) / 256;
+  // CTA pairs where they fill the SMs (dense) or an expert's rows fill their
+  // 256 rows on the average
+  const bool pair = g.tiles != nullptr ? g.mean_rows >= 256 : (g.rows + 255) / 256 * n_tiles >= sm_count() / 2;
+  // 64-column tiles where 256-column ones leave half of the SMs idle: 512 x
+  // 2048 x 1024 then takes 64 CTAs instead of 16
+  const bool narrow = !swiglu && g.tiles == nullptr && !pair && (g.rows + 127) / 128 * n_tiles <= sm_count() / 2;
   Fp8GemmParams p;
   memset(&p, 0, sizeof(p));
   int rc = fp8_map(&p.tmap_a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, g.q, g.rows, g.k, 128);
   if (rc) return rc;
-  rc = fp8_map(&p.tmap_b, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, g.wq, (int64_t)g.experts * g.n, g.k, 128);
+  rc = fp8_map(&p.tmap_b, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, g.wq, (int64_t)g.experts * g.n, g.k, narrow ? 64 : 128);
   if (rc) return rc;
-  const bool swiglu = g.out == nullptr;
   if (!swiglu && g.n % 8 == 0 && ((uintptr_t)g.out & 15) == 0) {
     rc = fp8_map(&p.tmap_out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, g.out, g.rows, g.n, 32);
     if (rc) return rc;
@@ -1051,14 +1070,13 @@ int run_fp8_gemm(const Fp8Gemm& g, cudaStream_t stream) {
   p.hq = g.hq;
   p.hs = g.hs;
   p.hs_ld = g.hs_ld;
-  const int64_t n_tiles = swiglu ? g.n / 256 : (g.n + 255) / 256;
-  const bool pair = g.tiles != nullptr ? g.mean_rows >= 256 : (g.rows + 255) / 256 * n_tiles >= sm_count() / 2;
   p.tiles = g.tiles == nullptr ? nullptr : pair ? g.tiles + g.max_tiles : g.tiles;
   const int64_t m_tiles = g.tiles != nullptr ? g.max_tiles : (g.rows + (pair ? 255 : 127)) / (pair ? 256 : 128);
-  const int64_t units = m_tiles * n_tiles;
+  const int64_t units = m_tiles * (narrow ? (g.n + 63) / 64 : n_tiles);
   if (swiglu)
-    return pair ? fp8_launch<2, FP8_SWIGLU>(p, units, stream) : fp8_launch<1, FP8_SWIGLU>(p, units, stream);
-  return pair ? fp8_launch<2, FP8_PLAIN>(p, units, stream) : fp8_launch<1, FP8_PLAIN>(p, units, stream);
+    return pair ? fp8_launch<2, 256, FP8_SWIGLU>(p, units, stream) : fp8_launch<1, 256, FP8_SWIGLU>(p, units, stream);
+  if (narrow) return fp8_launch<1, 64, FP8_PLAIN>(p, units, stream);
+  return pair ? fp8_launch<2, 256, FP8_PLAIN>(p, units, stream) : fp8_launch<1, 256, FP8_PLAIN>(p, units, stream);
 }
 
 constexpr size_t kFp8StreamSmemMax = 160 * 1024;

@@ -147,32 +147,41 @@ __global__ void __launch_bounds__(256) fp8_pack_kernel(const uint16_t* __restric
 }
 
 // ---------------------------------------------------------------------------
-// GEMM on tcgen05, 128 x 256 of the output per CTA (CTAS = 1) or 256 x 256 per
-// CTA pair (CTAS = 2, cta_group::2: each CTA holds its 128 rows and half of
-// the weight rows, so a k-block brings 32 KB per SM instead of 48).
+// GEMM on tcgen05: 128 x 256 of the output per CTA (or 128 x 64, see below), one
+// CTA per SM, persistent over the output tiles.
 //
 // warp 0      TMA producer: per k-block of 128 columns the A rows and the
 //             weight rows (128-byte swizzle)
-// warp 1      MMA issuer (leader CTA): per k-block one group of 4 MMAs into one
-//             of the two tensor-memory buffers of 256 columns
+// warp 1      MMA issuer: per k-block one group of 4 MMAs into one of the
+//             tensor-memory buffers (two of 256 columns, four of 64)
 // warp 2      relay: waits for a group's commit and meets the epilogue warps at
 //             a named barrier
-// warp 3      relay of the pair's second CTA: tells the leader that its epilogue
-//             has read a buffer
-// warps 4..11 epilogue: two warps per lane quadrant, 128 of the 256 columns
-//             each. Per k-block a thread reads its row's 128 columns in eight
-//             loads, the next in flight while it adds the last, times sx * sw,
-//             to 128 registers, and gives the buffer back as soon as it is read.
+// warp 3      relay: waits for a k-block's operands and meets the issuer and the
+//             epilogue (which has read the buffer) at a named barrier
+// warps 4..   epilogue: two warps per lane quadrant (one for 64 columns). Per
+//             k-block a thread reads its row's columns 16 at a time, the next
+//             load in flight while it adds the last, times sx * sw, to its
+//             registers, and gives the buffer back as soon as it is read.
 //
 // A buffer's round trip (products 512 clocks, commit, sums 260, release, next
 // issue) decides the rate, and what the warps wait on decides the round trip:
-// with one CTA and operands at rest a k-block takes 620 clocks where the
-// epilogue and the issuer meet at named barriers, 805 where every epilogue warp
-// waits on the commit's mbarrier and arrives on another, 680 and 900 with 16
-// epilogue warps of 64 columns.
+// with operands at rest a k-block takes 620 clocks where the epilogue and the
+// issuer meet at named barriers, 805 where every epilogue warp waits on the
+// commit's mbarrier and arrives on another (680 and 900 with 16 epilogue warps
+// of 64 columns). An mbarrier wait or a second commit in the issuer's loop
+// delays its next MMA by 100 to 200 clocks, hence the relays and one commit per
+// k-block, which frees the stage and announces the sums at once.
 //
-// Bound: 128 x 256 x 128 products are 512 clocks of one SM's tensor core; the
-// FMAs of the 128 x 256 block sums are 256 clocks of its fp32 lanes.
+// Bound: 128 x 256 x 128 products are 512 clocks of the tensor core, its operand
+// reads and the TMA writes of a k-block 768 clocks of shared memory, the FMAs of
+// the block sums 256 clocks of the fp32 lanes; 880 clocks are reached. CTA pairs
+// (cta_group::2, 256 x 256) need 512 clocks of shared memory but two more hops
+// across the cluster per buffer: 950 clocks, and 948 against 878 us for 16384
+// tokens through 4 of 64 experts (C 2048, F 1536). In a row of calls both hold
+// the card at its power limit (990 W, 1.6 GHz).
+//
+// 64-column tiles (four buffers, one epilogue warp per quadrant) are for
+// outputs whose 256-column tiles leave most SMs idle.
 // ---------------------------------------------------------------------------
 enum Fp8Mode : int { FP8_PLAIN = 0, FP8_SWIGLU = 1 };
 
@@ -183,7 +192,7 @@ struct Fp8GemmParams {
   const float* xs;       // activation scales, [K blocks][xs_ld]
   int64_t xs_ld;
   const float* ws;       // weight scales [E][N blocks][K blocks]
-  const TileEntry* tiles;    // grouped: table of 128-row tiles (CTAS = 1) or 256-row pairs; nullptr: dense rows
+  const TileEntry* tiles;    // grouped: table of 128-row tiles; nullptr: dense rows
   const int32_t* num_tiles;
   int64_t rows;          // rows of the activations and of the output
   int32_t N;             // weight rows per expert (2F for FP8_SWIGLU)
@@ -201,12 +210,12 @@ constexpr uint32_t kFp8BarMax = 1;   // SwiGLU row maxima: the epilogue warps
 constexpr uint32_t kFp8BarSums = 2;  // a buffer holds its block sums: relay -> epilogue
 constexpr uint32_t kFp8BarGo = 6;    // a buffer is read and its next operands are there: epilogue, relay -> issuer
 
-template <int CTAS, int BN>
+template <int BN>
 struct Fp8Shape {
   static constexpr int A_BYTES = 128 * 128;
-  static constexpr int B_BYTES = BN / CTAS * 128;
+  static constexpr int B_BYTES = BN * 128;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr int STAGES = BN == 64 ? 8 : CTAS == 2 ? 6 : 4;
+  static constexpr int STAGES = BN == 64 ? 8 : 4;
   static constexpr int BUFS = BN == 64 ? 4 : 2;  // tensor-memory buffers of BN columns
   static constexpr int OUT_BOX = 4096;           // 32 rows x 64 bf16 per epilogue warp
   static constexpr int EPI_WARPS = BN == 64 ? 4 : 8;
@@ -223,7 +232,7 @@ struct Fp8Shape {
                 "register split");
   static constexpr size_t SMEM_BYTES = 1024 + (size_t)STAGES * STAGE_BYTES + EPI_WARPS * OUT_BOX + 256;
   static_assert(SMEM_BYTES <= 232448, "shared memory budget");
-  static_assert(8 * (2 * STAGES + 3) <= 256 && BUFS <= 4, "barriers");
+  static_assert(8 * (2 * STAGES + 1) <= 256 && BUFS <= 4, "barriers");
 };
 
 // E4M3 x E4M3 -> F32 (kind::f8f6f4), K-major operands, K = 32 per MMA.
@@ -235,29 +244,15 @@ __host__ __device__ constexpr uint32_t idesc_e4m3(uint32_t m, uint32_t n) {
 
 // The high word of a descriptor is the same for every operand here; the low
 // word (the address) moves by 2 per 32 bytes.
-template <int CTAS, int ACCUMULATE>
+template <int ACCUMULATE>
 __device__ __forceinline__ void tc_mma_e4m3(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t desc_hi,
                                             uint32_t idesc) {
-  if constexpr (CTAS == 1)
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %5, 0;\n\t"
-        "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
-        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %4, p;\n\t}" ::"r"(d_tmem),
-        "r"(a_lo), "r"(b_lo), "r"(desc_hi), "r"(idesc), "n"(ACCUMULATE)
-        : "memory");
-  else
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %5, 0;\n\t"
-        "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
-        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], a, b, %4, p;\n\t}" ::"r"(d_tmem),
-        "r"(a_lo), "r"(b_lo), "r"(desc_hi), "r"(idesc), "n"(ACCUMULATE)
-        : "memory");
-}
-
-template <int CTAS>
-__device__ __forceinline__ void fp8_commit(uint64_t* bar) {
-  if constexpr (CTAS == 1) tc_commit(bar);
-  else tc_commit_pair(bar, 0x3);
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %5, 0;\n\t"
+      "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %4, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_lo), "r"(b_lo), "r"(desc_hi), "r"(idesc), "n"(ACCUMULATE)
+      : "memory");
 }
 
 // acc[0..15] += f * (the 16 columns in r). The statements are volatile, so they
@@ -309,15 +304,14 @@ __device__ __forceinline__ void regs_down() {
 }
 
 // Row tile m of the launch: dense rows, or the table's entry.
-template <int CTAS>
 __device__ __forceinline__ TileEntry fp8_tile(const Fp8GemmParams& p, int m) {
   if (p.tiles != nullptr) {
     return p.tiles[m];
   }
   TileEntry t;
   t.expert = 0;
-  t.row0 = m * CTAS * kTileRows;
-  t.valid = (int32_t)min((int64_t)CTAS * kTileRows, p.rows - t.row0);
+  t.row0 = m * kTileRows;
+  t.valid = (int32_t)min((int64_t)kTileRows, p.rows - t.row0);
   t.pad = 0;
   return t;
 }
@@ -340,11 +334,12 @@ __device__ constexpr uint32_t chunk_col(int c) {
   return 16 * c + (MODE == FP8_SWIGLU && c >= 4 ? 64 : 0);
 }
 
-template <int CTAS, int BN, int MODE>
-__device__ __forceinline__ void fp8_gemm_body(const Fp8GemmParams& p) {
+template <int BN, int MODE>
+__global__ void __launch_bounds__(Fp8Shape<BN>::THREADS, 1)
+    fp8_gemm_kernel(const __grid_constant__ Fp8GemmParams p) {
   pdl_wait();  // the previous kernel of the stream has completed
   pdl_trigger();
-  using S = Fp8Shape<CTAS, BN>;
+  using S = Fp8Shape<BN>;
   static_assert(MODE == FP8_PLAIN || BN == 256, "a SwiGLU tile is one block of 128 hidden columns");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -353,20 +348,17 @@ __device__ __forceinline__ void fp8_gemm_body(const Fp8GemmParams& p) {
   uint8_t* sOut = sB + S::STAGES * S::B_BYTES;
   float* s_max = reinterpret_cast<float*>(sOut);  // FP8_SWIGLU: row maxima [unit parity][half][row]
   uint64_t* full = reinterpret_cast<uint64_t*>(sOut + S::EPI_WARPS * S::OUT_BOX);
-  uint64_t* done = full + S::STAGES;       // products of a stage complete: its sums are there, its memory is free
-  uint64_t* peer_free = done + S::STAGES;  // per buffer, the leader's: its peer has read it
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(peer_free + 2);
+  uint64_t* done = full + S::STAGES;  // products of a stage complete: its sums are there, its memory is free
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + S::STAGES);
 
   const int warp = threadIdx.x >> 5;
   const uint32_t lane = threadIdx.x & 31;
-  const uint32_t rank = CTAS == 1 ? 0u : cluster_ctarank();
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S::STAGES; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&done[s], 1);
     }
-    for (int b = 0; b < 2; ++b) mbar_init(&peer_free[b], S::EPI_WARPS);
     fence_barrier_init();
   }
   if (warp == 0 && lane == 0) {
@@ -374,28 +366,22 @@ __device__ __forceinline__ void fp8_gemm_body(const Fp8GemmParams& p) {
     tma_prefetch_desc(&p.tmap_b);
   }
   if (warp == 1) {
-    if constexpr (CTAS == 1) {
-      tmem_alloc(tmem_slot, S::BUFS * BN);
-      tmem_relinquish();
-    } else {
-      tmem_alloc_pair(tmem_slot, 512);
-      tmem_relinquish_pair();
-    }
+    tmem_alloc(tmem_slot, S::BUFS * BN);
+    tmem_relinquish();
   }
   __syncwarp();
   tc_fence_before();
-  if constexpr (CTAS == 1) __syncthreads();
-  else cluster_sync();  // barriers of both CTAs initialised before any cross-CTA signal
+  __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
   const int F = p.N / 2;
   const int n_tiles = MODE == FP8_SWIGLU ? F / 128 : (p.N + BN - 1) / BN;
   const int num_m =
-      p.tiles != nullptr ? p.num_tiles[CTAS - 1] : (int)((p.rows + CTAS * kTileRows - 1) / (CTAS * kTileRows));
+      p.tiles != nullptr ? p.num_tiles[0] : (int)((p.rows + kTileRows - 1) / kTileRows);
   const int total = num_m * n_tiles;
   const int k_blocks = (p.K + kFp8Block - 1) / kFp8Block;
-  const int first = blockIdx.x / CTAS, step = gridDim.x / CTAS;
+  const int first = blockIdx.x, step = gridDim.x;
   // k-blocks of this CTA: every role below takes exactly this many turns, on
   // every path, so that the named barriers stay matched (the issuer commits
   // each turn, so the waits for its commits end too)
@@ -404,10 +390,9 @@ __device__ __forceinline__ void fp8_gemm_body(const Fp8GemmParams& p) {
   if (warp < S::EPI_WARP0) {
     if constexpr (S::SPLIT_REGS) regs_down<S::FRONT_REGS>();
     if (warp == 0) {
-      // ---------------- TMA producer (every CTA) ----------------
-      // one lane per copy: A, the weight rows, of 256 in two copies (CTAS = 1)
-      const uint32_t full_leader = CTAS == 1 ? 0u : mapa_shared(smem_u32(full), 0);
-      constexpr uint32_t kCopies = CTAS == 1 && BN == 256 ? 3 : 2;
+      // ---------------- TMA producer ----------------
+      // one lane per copy: A, the weight rows, of 256 in two copies
+      constexpr uint32_t kCopies = BN == 256 ? 3 : 2;
       const CUtensorMap* map = lane == 0 ? &p.tmap_a : &p.tmap_b;
       uint8_t* const dst0 = lane == 0 ? sA : sB + (lane == 2 ? 16384 : 0);
       const uint32_t dst_step = lane == 0 ? S::A_BYTES : S::B_BYTES;
@@ -415,31 +400,26 @@ __device__ __forceinline__ void fp8_gemm_body(const Fp8GemmParams& p) {
       bool ok = true;
       for (int u = first; u < total && ok; u += step) {
         const int m = u / n_tiles, n = u - m * n_tiles;
-        const TileEntry t = fp8_tile<CTAS>(p, m);
-        // weight rows of columns 0..127 and 128..255 (of the leader and its peer)
-        const int part = CTAS == 1 ? (lane == 2 ? 1 : 0) : (int)rank;
-        const int row = lane == 0 ? t.row0 + 128 * (int)rank
+        const TileEntry t = fp8_tile(p, m);
+        const int part = lane == 2 ? 1 : 0;  // weight rows of columns 0..127, 128..255
+        const int row = lane == 0 ? t.row0
                                   : t.expert * p.N + (MODE == FP8_SWIGLU ? n * 128 + part * F : n * BN + part * 128);
         for (int kb = 0; kb < k_blocks; ++kb) {
           ok = fp8_wait(&done[stage], phase ^ 1u, kErrTimeoutProducer);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
-          if (rank == 0 && lane == 0) mbar_arrive_expect_tx(&full[stage], CTAS * S::STAGE_BYTES);
+          if (lane == 0) mbar_arrive_expect_tx(&full[stage], S::STAGE_BYTES);
           __syncwarp();
-          if (lane < kCopies) {
-            uint8_t* dst = dst0 + stage * dst_step;
-            if constexpr (CTAS == 1) tma_load_2d(dst, map, &full[stage], kb * 128, row);
-            else tma_load_2d_pair(dst, map, full_leader + stage * 8, kb * 128, row);
-          }
+          if (lane < kCopies) tma_load_2d(dst0 + stage * dst_step, map, &full[stage], kb * 128, row);
           if (++stage == S::STAGES) {
             stage = 0;
             phase ^= 1u;
           }
         }
       }
-    } else if (warp == 1 && rank == 0) {
-      // ---------------- MMA issuer (leader) ----------------
-      constexpr uint32_t idesc = idesc_e4m3(128 * CTAS, BN);
+    } else if (warp == 1) {
+      // ---------------- MMA issuer ----------------
+      constexpr uint32_t idesc = idesc_e4m3(128, BN);
       const uint64_t a_desc = smem_desc(smem_u32(sA), 16, 1024, kLayoutSwizzle128B);
       const uint32_t desc_hi = (uint32_t)(a_desc >> 32), a_lo = (uint32_t)a_desc;
       const uint32_t b_lo = (uint32_t)smem_desc(smem_u32(sB), 16, 1024, kLayoutSwizzle128B);
@@ -450,11 +430,11 @@ __device__ __forceinline__ void fp8_gemm_body(const Fp8GemmParams& p) {
         if (lane == 0) {
           const uint32_t a = a_lo + stage * (S::A_BYTES >> 4), b = b_lo + stage * (S::B_BYTES >> 4);
           const uint32_t d = tmem + buf * BN;
-          tc_mma_e4m3<CTAS, 0>(d, a, b, desc_hi, idesc);
-          tc_mma_e4m3<CTAS, 1>(d, a + 2, b + 2, desc_hi, idesc);
-          tc_mma_e4m3<CTAS, 1>(d, a + 4, b + 4, desc_hi, idesc);
-          tc_mma_e4m3<CTAS, 1>(d, a + 6, b + 6, desc_hi, idesc);
-          fp8_commit<CTAS>(&done[stage]);
+          tc_mma_e4m3<0>(d, a, b, desc_hi, idesc);
+          tc_mma_e4m3<1>(d, a + 2, b + 2, desc_hi, idesc);
+          tc_mma_e4m3<1>(d, a + 4, b + 4, desc_hi, idesc);
+          tc_mma_e4m3<1>(d, a + 6, b + 6, desc_hi, idesc);
+          tc_commit(&done[stage]);
         }
         __syncwarp();
         if (++stage == S::STAGES) stage = 0;
@@ -464,7 +444,7 @@ __device__ __forceinline__ void fp8_gemm_body(const Fp8GemmParams& p) {
       for (int i = turns < S::BUFS ? 0 : turns - S::BUFS; i < turns; ++i)
         named_sync(kFp8BarGo + i % S::BUFS, 32 * (S::EPI_WARPS + 2));
     } else if (warp == 2) {
-      // ---------------- relay: products complete -> epilogue (every CTA) ----------------
+      // ---------------- relay: products complete -> epilogue ----------------
       uint32_t stage = 0, phase = 0;
       for (int i = 0; i < turns; ++i) {
         fp8_wait(&done[stage], phase, kErrTimeoutEpilogue, 2000000000ull, false);
@@ -475,40 +455,34 @@ __device__ __forceinline__ void fp8_gemm_body(const Fp8GemmParams& p) {
           phase ^= 1u;
         }
       }
-    } else if (warp == 3 && rank == 0) {
-      // ---------------- relay: operands landed, peer's buffer read -> issuer (leader) ----------------
-      // takes part in the go barrier for what would be waits of the issuer
-      uint32_t stage = 0, stage_phase = 0, buf = 0, phase = 0;
+    } else {
+      // ---------------- relay: operands landed -> issuer ----------------
+      // takes part in the go barrier for what would be a wait of the issuer
+      uint32_t stage = 0, stage_phase = 0, buf = 0;
       bool ok = true;
       for (int i = 0; i < turns; ++i) {
         ok = ok && fp8_wait(&full[stage], stage_phase, kErrTimeoutMma);
-        if (CTAS == 2 && i >= S::BUFS) fp8_wait(&peer_free[buf], phase ^ 1u, kErrTimeoutMma, 2000000000ull, false);
         __syncwarp();
         named_sync(kFp8BarGo + buf, i < S::BUFS ? 64 : 32 * (S::EPI_WARPS + 2));
         if (++stage == S::STAGES) {
           stage = 0;
           stage_phase ^= 1u;
         }
-        if (++buf == S::BUFS) {
-          buf = 0;
-          phase ^= 1u;
-        }
+        if (++buf == S::BUFS) buf = 0;
       }
       for (int i = turns < S::BUFS ? 0 : turns - S::BUFS; i < turns; ++i)
         named_sync(kFp8BarGo + i % S::BUFS, 32 * (S::EPI_WARPS + 2));
     }
   } else {
     if constexpr (S::SPLIT_REGS) regs_up<S::EPI_REGS>();
-    // ---------------- epilogue (warps 4..19, every CTA) ----------------
+    // ---------------- epilogue ----------------
     const uint32_t quad = (uint32_t)(warp & 3);
     const int h = (warp - S::EPI_WARP0) >> 2;  // columns COLS h .. (SwiGLU: gate 64 h .. and up 128 + 64 h ..)
-    const int row_in_cta = (int)(quad * 32 + lane);
-    const uint32_t peer_free_leader = CTAS == 1 ? 0u : mapa_shared(smem_u32(peer_free), 0);
+    const int row_in_tile = (int)(quad * 32 + lane);
     const uint32_t taddr = tmem + ((quad * 32u) << 16) + (MODE == FP8_SWIGLU ? 64u : (uint32_t)S::COLS) * h;
     const int n_blocks = (p.N + kFp8Block - 1) / kFp8Block;
     // A unit's rows, columns and scale addresses, and the scales of its first
     // two k-blocks, are fetched while the previous unit is written out.
-    const int row_in_tile = row_in_cta + 128 * (int)rank;
     const int64_t up = MODE == FP8_SWIGLU ? (int64_t)(F / 128) * k_blocks : 0;
     int n = 0, valid = 0;
     int64_t row = 0;
@@ -516,7 +490,7 @@ __device__ __forceinline__ void fp8_gemm_body(const Fp8GemmParams& p) {
     float x0 = 0.0f, w00 = 0.0f, w01 = 0.0f, x1 = 0.0f, w10 = 0.0f, w11 = 0.0f;
     auto fetch = [&](int u) {
       const int m = u / n_tiles;
-      const TileEntry t = fp8_tile<CTAS>(p, m);
+      const TileEntry t = fp8_tile(p, m);
       n = u - m * n_tiles;
       valid = t.valid;
       row = (int64_t)t.row0 + row_in_tile;
@@ -567,12 +541,7 @@ __device__ __forceinline__ void fp8_gemm_body(const Fp8GemmParams& p) {
         }
         tc_wait_ld();
         tc_fence_before();
-        if (CTAS == 1 || rank == 0) {
-          named_arrive(kFp8BarGo + buf, 32 * (S::EPI_WARPS + 2));
-        } else {
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(peer_free_leader + buf * 8);
-        }
+        named_arrive(kFp8BarGo + buf, 32 * (S::EPI_WARPS + 2));
         fp8_add_block(acc + S::COLS - 16, rb, f1);
         if (++buf == S::BUFS) buf = 0;
       }
@@ -589,7 +558,7 @@ __device__ __forceinline__ void fp8_gemm_body(const Fp8GemmParams& p) {
           swiglu_pair_f32(acc[j], acc[j + 1], acc[64 + j], acc[65 + j]);
           a = fmaxf(a, fmaxf(fabsf(acc[j]), fabsf(acc[j + 1])));
         }
-        float* mx = s_max + (unit & 1u) * 256 + row_in_cta;
+        float* mx = s_max + (unit & 1u) * 256 + row_in_tile;
         mx[h * 128] = a;
         named_sync(kFp8BarMax, 32 * S::EPI_WARPS);
         a = fmaxf(a, mx[(h ^ 1) * 128]);
@@ -613,7 +582,7 @@ __device__ __forceinline__ void fp8_gemm_body(const Fp8GemmParams& p) {
         const int col0 = n_out * BN + S::COLS * h;
         // boxes of 32 rows x 64 columns in the TMA 128-byte swizzle
         uint8_t* box = sOut + (warp - S::EPI_WARP0) * S::OUT_BOX;
-        const int box_rows = valid_out - 128 * (int)rank - 32 * (int)quad;  // rows of the box that exist
+        const int box_rows = valid_out - 32 * (int)quad;  // rows of the box that exist
 #pragma unroll
         for (int i = 0; i < S::COLS / 64; ++i) {
           const int col = col0 + 64 * i;
@@ -659,25 +628,11 @@ __device__ __forceinline__ void fp8_gemm_body(const Fp8GemmParams& p) {
 
   __syncwarp();
   tc_fence_before();
-  if constexpr (CTAS == 1) __syncthreads();
-  else cluster_sync();  // all tensor-memory reads and cross-CTA signals of the pair done
+  __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    if constexpr (CTAS == 1) tmem_dealloc(tmem, S::BUFS * BN);
-    else tmem_dealloc_pair(tmem, 512);
+    tmem_dealloc(tmem, S::BUFS * BN);
   }
-}
-
-template <int BN, int MODE>
-__global__ void __launch_bounds__(Fp8Shape<1, BN>::THREADS, 1)
-    fp8_gemm_kernel(const __grid_constant__ Fp8GemmParams p) {
-  fp8_gemm_body<1, BN, MODE>(p);
-}
-
-template <int MODE>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Fp8Shape<2, 256>::THREADS, 1)
-    fp8_gemm_pair_kernel(const __grid_constant__ Fp8GemmParams p) {
-  fp8_gemm_body<2, 256, MODE>(p);
 }
 
 // ---------------------------------------------------------------------------
@@ -950,16 +905,12 @@ static int fp8_map(CUtensorMap* map, CUtensorMapDataType type, int elem, const v
   return PRAXIS_B200_OK;
 }
 
-// Launches on at most one CTA (pair) per SM; `units` bounds the work.
-template <int CTAS, int BN, int MODE>
+// Launches on at most one CTA per SM; `units` bounds the work.
+template <int BN, int MODE>
 static int fp8_launch(const Fp8GemmParams& p, int64_t units, cudaStream_t stream) {
-  using S = Fp8Shape<CTAS, BN>;
-  auto kernel = [] {
-    if constexpr (CTAS == 1) return fp8_gemm_kernel<BN, MODE>;
-    else return fp8_gemm_pair_kernel<MODE>;
-  }();
+  using S = Fp8Shape<BN>;
+  auto kernel = fp8_gemm_kernel<BN, MODE>;
   static DeviceOnce attr;
-  static int max_groups[kMaxDevices] = {0};
   const int rc = device_once(attr, [&](int dev) {
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM_BYTES);
     if (e != cudaSuccess)
@@ -970,30 +921,11 @@ static int fp8_launch(const Fp8GemmParams& p, int64_t units, cudaStream_t stream
     if (e != cudaSuccess || (S::SPLIT_REGS && fa.numRegs < S::LAUNCH_REGS))
       return set_error(PRAXIS_B200_ECUDA, "fp8 gemm: built with %d registers a thread, needs %d", fa.numRegs,
                        S::LAUNCH_REGS);
-    int n = sm_count();
-    if (CTAS == 2) {
-      cudaLaunchConfig_t cfg = {};
-      cfg.gridDim = dim3(2 * (sm_count() / 2));
-      cfg.blockDim = dim3(S::THREADS);
-      cfg.dynamicSmemBytes = S::SMEM_BYTES;
-      cudaLaunchAttribute a;
-      a.id = cudaLaunchAttributeClusterDimension;
-      a.val.clusterDim.x = 2;
-      a.val.clusterDim.y = 1;
-      a.val.clusterDim.z = 1;
-      cfg.attrs = &a;
-      cfg.numAttrs = 1;
-      e = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg);
-      if (e != cudaSuccess || n <= 0) n = sm_count() / 2;
-    }
-    max_groups[dev] = n;
     return (int)PRAXIS_B200_OK;
   });
   if (rc) return rc;
-  int dev = 0;
-  cudaGetDevice(&dev);
-  const int groups = (int)(units < max_groups[dev] ? units : max_groups[dev]);
-  launch_pdl(kernel, dim3(CTAS * groups), dim3(S::THREADS), S::SMEM_BYTES, stream, p);
+  const int grid = (int)(units < sm_count() ? units : sm_count());
+  launch_pdl(kernel, dim3(grid), dim3(S::THREADS), S::SMEM_BYTES, stream, p);
   return check_launch("fp8_gemm");
 }
 
@@ -1017,8 +949,7 @@ int run_fp8_pack(const uint16_t* w, int64_t experts, int64_t k, int64_t n, uint8
 
 // One GEMM over quantized rows. Dense (tiles == nullptr): `rows` rows against
 // one weight. Grouped: the dispatch's tables, rows = padded rows, max_tiles
-// bounds the 128-row tiles and mean_rows is the mean number of routed rows per
-// expert. out (FP8_PLAIN) or hq / hs (FP8_SWIGLU) get the result.
+// bounds the 128-row tiles. out (FP8_PLAIN) or hq / hs (FP8_SWIGLU) get the result.
 struct Fp8Gemm {
   const uint8_t* q;
   const float* xs;
@@ -1030,7 +961,6 @@ struct Fp8Gemm {
   const TileEntry* tiles;
   const int32_t* num_tiles;
   int32_t max_tiles;
-  int64_t mean_rows;
   uint16_t* out;
   uint8_t* hq;
   float* hs;
@@ -1041,12 +971,10 @@ int run_fp8_gemm(const Fp8Gemm& g, cudaStream_t stream) {
   if (g.rows == 0) return PRAXIS_B200_OK;
   const bool swiglu = g.out == nullptr;
   const int64_t n_tiles = swiglu ? g.n / 256 : (g.n + 255) / 256;
-  // CTA pairs where they fill the SMs (dense) or an expert's rows fill their
-  // 256 rows on the average
-  const bool pair = g.tiles != nullptr ? g.mean_rows >= 256 : (g.rows + 255) / 256 * n_tiles >= sm_count() / 2;
-  // 64-column tiles where 256-column ones leave half of the SMs idle: 512 x
-  // 2048 x 1024 then takes 64 CTAs instead of 16
-  const bool narrow = !swiglu && g.tiles == nullptr && !pair && (g.rows + 127) / 128 * n_tiles <= sm_count() / 2;
+  const int64_t m_tiles = g.tiles != nullptr ? g.max_tiles : (g.rows + 127) / 128;
+  // 64-column tiles where they all fit the SMs at once (K = 4096, cold weights:
+  // 32 tiles of 256 columns 21 us, the same in 64 columns 18; 64 tiles 23 against 28)
+  const bool narrow = !swiglu && g.tiles == nullptr && 4 * m_tiles * n_tiles <= sm_count();
   Fp8GemmParams p;
   memset(&p, 0, sizeof(p));
   int rc = fp8_map(&p.tmap_a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, g.q, g.rows, g.k, 128);
@@ -1070,13 +998,10 @@ int run_fp8_gemm(const Fp8Gemm& g, cudaStream_t stream) {
   p.hq = g.hq;
   p.hs = g.hs;
   p.hs_ld = g.hs_ld;
-  p.tiles = g.tiles == nullptr ? nullptr : pair ? g.tiles + g.max_tiles : g.tiles;
-  const int64_t m_tiles = g.tiles != nullptr ? g.max_tiles : (g.rows + (pair ? 255 : 127)) / (pair ? 256 : 128);
-  const int64_t units = m_tiles * (narrow ? (g.n + 63) / 64 : n_tiles);
-  if (swiglu)
-    return pair ? fp8_launch<2, 256, FP8_SWIGLU>(p, units, stream) : fp8_launch<1, 256, FP8_SWIGLU>(p, units, stream);
-  if (narrow) return fp8_launch<1, 64, FP8_PLAIN>(p, units, stream);
-  return pair ? fp8_launch<2, 256, FP8_PLAIN>(p, units, stream) : fp8_launch<1, 256, FP8_PLAIN>(p, units, stream);
+  p.tiles = g.tiles;
+  if (swiglu) return fp8_launch<256, FP8_SWIGLU>(p, m_tiles * n_tiles, stream);
+  if (narrow) return fp8_launch<64, FP8_PLAIN>(p, m_tiles * ((g.n + 63) / 64), stream);
+  return fp8_launch<256, FP8_PLAIN>(p, m_tiles * n_tiles, stream);
 }
 
 constexpr size_t kFp8StreamSmemMax = 160 * 1024;
@@ -1102,11 +1027,14 @@ static int fp8_stream_launch(const Fp8StreamParams& p, int groups, cudaStream_t 
 
 // Whether a product of `rows` rows goes through the streaming kernels: dense up
 // to the 8 rows that share a weight; routed slots read their expert's weight
-// each for itself, so as long as they are few. The quantized rows have to fit
+// each for itself, so as long as they are few (C 2048, F 1536, 64 experts, cold
+// weights: 16 slots 48 us, through the dispatch and the tiles above 59; 32 slots
+// 75 against 86, 64 slots 134 against 113; 8 experts, C 1024, F 2048: 16 slots
+// 35 against 37, 24 slots 49 against 37). The quantized rows have to fit
 // the shared memory (k_up: columns of the rows, k_down: of the hidden rows, 0
 // for a linear product).
 static bool fp8_streams(int64_t rows, int top_k, int experts, int k_up, int k_down) {
-  if (top_k == 0 ? rows > 8 : rows * top_k > 16 && rows * top_k > (experts < 64 ? experts : 64)) return false;
+  if (top_k == 0 ? rows > 8 : rows * top_k > 16 && rows * top_k > experts / 2) return false;
   return fp8_stream_smem(top_k == 0 ? (int)rows : 1, k_up) <= kFp8StreamSmemMax &&
          fp8_stream_smem(top_k == 0 ? (int)rows : top_k, k_down) <= kFp8StreamSmemMax;
 }

@@ -175,7 +175,7 @@ def check_linear(y, x, q, s):
 LINEAR = [(1, 1, 16), (1, 256, 128), (1, 4096, 2048), (2, 129, 272), (3, 7, 48), (5, 1000, 400), (8, 512, 128),
           (9, 640, 1024), (16, 1001, 1040), (17, 264, 512), (33, 2048, 256), (64, 136, 384), (77, 1001, 1040),
           (128, 128, 128), (129, 257, 144), (255, 384, 1152), (300, 512, 2048), (513, 1030, 272), (1000, 4096, 512),
-          (2100, 2312, 784)]
+          (2100, 2312, 784), (1100, 2501, 272), (8, 40, 24576), (1, 33, 32768)]
 
 
 @pytest.mark.parametrize("m,n,k", LINEAR)
@@ -270,7 +270,8 @@ def test_linear_refuses_at_the_c_level(P):
 # -- feed-forward ----------------------------------------------------------------
 
 @pytest.mark.parametrize("m,c,f", [(1, 128, 128), (1, 1024, 512), (5, 256, 384), (16, 384, 128), (70, 256, 640),
-                                   (128, 512, 256), (300, 640, 384), (1100, 256, 512)])
+                                   (128, 512, 256), (300, 640, 384), (1100, 256, 512),
+                                   (2600, 128, 1024)])
 def test_mlp(P, m, c, f):
     g = gen(m + c + f)
     gu, down = weight(g, 2 * f, c), weight(g, c, f)
@@ -296,7 +297,8 @@ def routing(g, t, e, k, kind):
 EXPERTS = [(1, 256, 128, 8, 8, ""), (1, 512, 384, 64, 4, ""), (3, 128, 256, 8, 2, "few"), (7, 256, 128, 4, 1, ""),
            (16, 384, 256, 16, 4, "skewed"), (33, 256, 384, 32, 6, ""), (40, 256, 256, 3, 2, "few"),
            (130, 256, 128, 5, 2, "skewed"), (257, 384, 256, 8, 3, ""), (900, 256, 384, 4, 2, ""),
-           (1500, 128, 128, 2, 1, "skewed"), (700, 256, 256, 160, 8, "")]
+           (1500, 128, 128, 2, 1, "skewed"), (700, 256, 256, 160, 8, ""),
+           (4000, 256, 512, 8, 2, "skewed")]
 
 
 @pytest.mark.parametrize("t,c,f,e,k,kind", EXPERTS)
@@ -381,6 +383,35 @@ def test_bank_chunks_and_tail(P):
     tail = P.ops.Tail(residual)
     new, normed = bank.routed_forward_tail(x, top, gate, scaling=2.5, chunk_size=t, tail=tail, shared=shared)
     assert normed is None and torch.equal(new, residual + both)
+
+
+def test_offsets_past_32_bits(P):
+    """Weights of more than 2^32 bytes and activations of more than 2^32."""
+    e, c, f = 65, 8192, 4096
+    g = torch.Generator(device=DEV).manual_seed(25)
+
+    def bank(*shape):
+        q = torch.randint(0, 120, shape, generator=g, device=DEV, dtype=torch.uint8).view(F8)
+        return q, torch.rand(shape[0], shape[1] // 128, shape[2] // 128, generator=g, device=DEV) * 1e-4
+
+    gu, down = bank(e, 2 * f, c), bank(e, c, f)
+    assert gu[0].numel() > 2**32
+    last = tuple(w[e - 1:].contiguous() for w in (*gu, *down))
+    for t in (3, 150):
+        x = torch.randn(t, c, generator=g, device=DEV).to(BF16)
+        top = torch.full((t, 1), e - 1, dtype=torch.int64, device=DEV)
+        gate = torch.ones(t, 1, dtype=BF16, device=DEV)
+        y = P.ops.fp8_moe_forward(x, top, gate, *gu, *down, 1.0)
+        assert same_bits(y, P.ops.fp8_moe_forward(x, top * 0, gate, *last, 1.0)) and bool(y.any())
+    del gu, down, last
+    rows, k = 2**32 // 8192 + 200, 8192
+    x = torch.randn(1000, k, generator=g, device=DEV).to(BF16)
+    q, s = weight(gen(26), 24, k)
+    big = torch.zeros(rows, k, dtype=BF16, device=DEV)
+    big[-1000:] = x
+    y = P.ops.fp8_linear(big, q, s)
+    check_linear(y[-1000:], x, q, s)
+    assert not y[:-1000].any()
 
 
 # -- the routing -----------------------------------------------------------------
@@ -539,6 +570,22 @@ def test_other_stream(P):
         lin = P.ops.fp8_linear(x, m.shared.gate_up_q, m.shared.gate_up_scale)
     side.synchronize()
     assert same_bits(got, want) and same_bits(lin, P.ops.fp8_linear(x, m.shared.gate_up_q, m.shared.gate_up_scale))
+
+
+def test_two_streams_at_once(P):
+    g = gen(51)
+    q, s = weight(g, 1024, 512)
+    xs = [randn(g, m, 512) for m in (3, 700)]
+    want = [P.ops.fp8_linear(x, q, s) for x in xs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in xs]
+    got = [[], []]
+    for _ in range(20):
+        for i, (x, stream) in enumerate(zip(xs, streams, strict=True)):
+            with torch.cuda.stream(stream):
+                got[i].append(P.ops.fp8_linear(x, q, s))
+    torch.cuda.synchronize()
+    assert all(same_bits(y, w) for ys, w in zip(got, want, strict=True) for y in ys)
 
 
 @pytest.mark.parametrize("t", [1, 12, 300])

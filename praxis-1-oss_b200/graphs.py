@@ -221,21 +221,22 @@ def enable_moe_cuda_graphs(modules, device=None, *, warmup: int = 3, max_graphs:
                            validate: bool = True) -> CudaGraphPool:
     """``enable_nvfp4_moe_cuda_graphs`` (praxis/cuda_graphs.py:245-283) for a
     set of MoE layers: every module whose routed bank is this library's (a
-    ``B200MoEFeedForward``, or a reference ``MoEFeedForward`` whose
-    ``routed`` was swapped for ``B200NVFP4RoutedExperts``) gets its
+    ``B200MoEFeedForward`` with NVFP4 or FP8 experts, or a reference
+    ``MoEFeedForward`` whose ``routed`` was swapped for one) gets its
     ``forward`` captured per input shape, with the routing, dispatch,
     quantization, GEMMs and combine inside one graph. ``modules``: a module
     (its MoE submodules are found by name) or an iterable of (name, module).
     Frozen eval modules only; their banks are prepared here."""
     from .bank import B200NVFP4RoutedExperts
+    from .fp8 import B200FP8RoutedExperts
 
     if isinstance(modules, nn.Module):
         found = [(n, m) for n, m in modules.named_modules()
-                 if isinstance(getattr(m, "routed", None), B200NVFP4RoutedExperts)]
+                 if isinstance(getattr(m, "routed", None), (B200NVFP4RoutedExperts, B200FP8RoutedExperts))]
     else:
         found = list(modules)
     if not found:
-        raise ValueError("no MoE layer with a B200 NVFP4 routed bank")
+        raise ValueError("no MoE layer with a B200 routed bank")
     for _, m in found:
         if m.training or any(p.requires_grad for p in m.parameters()):
             raise ValueError("MoE CUDA Graphs require frozen eval MoEs")

@@ -613,6 +613,22 @@ def test_two_captured_graphs_and_eager_calls(P, t):
             assert same_bits(got, w)
 
 
+@pytest.mark.parametrize("t", [1, 70])
+def test_captured_layer(P, t):
+    """The graph pool finds layers with FP8 experts and replays their forward."""
+    g = gen(80 + t)
+    m = layer(P, g).eval().requires_grad_(False)
+    xs = [randn(g, 1, t, 256) for _ in range(3)]
+    want = [m(x) for x in xs]
+    pool = P.graphs.enable_moe_cuda_graphs(torch.nn.ModuleList([m]), warmup=1)
+    try:
+        for x, y in zip(xs, want, strict=True):
+            assert same_bits(m(x), y)
+        assert [s["captures"] for s in pool.stats().values()] == [1]
+    finally:
+        pool.release()
+
+
 def test_torch_operators_match_direct_calls(P):
     g = gen(70)
     t, c, f, e, k = 30, 256, 128, 8, 2

@@ -818,7 +818,7 @@ def fp8_linear(x: Tensor, w_q: Tensor, w_scale: Tensor) -> Tensor:
     n, k = w_q.shape
     x, r, pitch = _fp8_rows(x, k)
     _on(x, device)
-    _inference_only(x)
+    _inference_only(x, w_q, w_scale)
     out = x.new_empty(x.shape[:-1] + (n,))
     lib = capi.load()
     size = lib.praxis_b200_fp8_linear_workspace_size(r, n, k)
@@ -875,7 +875,7 @@ def fp8_mlp(x: Tensor, gate_up_q: Tensor, gate_up_scale: Tensor, down_q: Tensor,
     if pitch != sizes[1]:
         raise ValueError("x: expected a contiguous CUDA bf16 tensor")
     _on(x, sizes[3])
-    _inference_only(x)
+    _inference_only(x, gate_up_q, gate_up_scale, down_q, down_scale)
     if out is None:
         out = torch.empty_like(x)
     else:
@@ -911,8 +911,8 @@ def fp8_moe_forward(x: Tensor, top_idx: Tensor, gate: Tensor, gate_up_q: Tensor,
         raise ValueError("top_idx / gate: expected [T, k], 1 <= k <= min(8, E)")
     if shared is not None and shared.shape != x.shape:
         raise ValueError("shared must have the shape of x")
-    _inference_only(x, gate, shared)
     weights = (gate_up_q, gate_up_scale, down_q, down_scale)
+    _inference_only(x, gate, shared, *weights)
     if tail is not None:
         st, residual_out, normed = _tail_struct(tail, t, c, x.device, tail_out)
         _fp8_ffn(x, t, top_idx, gate, shared, None, weights, sizes, float(scaling), st)

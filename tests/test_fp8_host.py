@@ -74,6 +74,8 @@ def test_products_refuse_gradients():
         q, s = weight(128, 256)
         with pytest.raises(RuntimeError, match="inference"):
             pkg().ops.fp8_linear(cuda(4, 256).requires_grad_(), q, s)
+        with pytest.raises(RuntimeError, match="inference"):
+            pkg().ops.fp8_linear(cuda(4, 256), q, s.requires_grad_())
 
 
 @pytest.mark.parametrize("kind", ["odd", "small", "down", "out", "x_strided", "experts"])

@@ -717,7 +717,8 @@ static int fp8_check(const char* what, int64_t rows, int64_t n, int64_t k) {
   if (rows < 0 || rows > 0x7fffff00ll || n < 1 || k < 16 || k % 16 != 0)
     return set_error(PRAXIS_B200_EINVAL, "%s: needs 0..2^31 rows, n >= 1 and a k that is a multiple of 16 (%lld, %lld, %lld)",
                      what, (long long)rows, (long long)n, (long long)k);
-  if (((rows + 127) / 128) * ((n + 255) / 256) > 0x7fffffffll)
+  // a tile's number and the next one of its CTA are 32-bit numbers
+  if (((rows + 127) / 128) * ((n + 255) / 256) > 0x7fff0000ll)
     return set_error(PRAXIS_B200_EINVAL, "%s: too many output tiles", what);
   return PRAXIS_B200_OK;
 }

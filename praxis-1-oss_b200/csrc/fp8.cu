@@ -266,9 +266,10 @@ __device__ __forceinline__ void fp8_add_block(float* acc, const uint32_t (&r)[16
 // mbar_wait (common.cuh) for waits on the path of every MMA: each try may
 // suspend the warp for up to 100 us of its own (polling warps take issue slots
 // and shared-memory cycles from the others), and the clock is read every 64
-// tries.
-__device__ __forceinline__ bool fp8_wait(uint64_t* bar, uint32_t parity, unsigned int code,
-                                         uint64_t limit_ns = 2000000000ull, bool stop_on_error = true) {
+// tries. An error that another kernel has left is no reason to give up: only
+// the limit ends the wait.
+__device__ __forceinline__ bool fp8_wait(uint64_t* bar, uint32_t parity, unsigned int code) {
+  constexpr uint64_t limit_ns = 2000000000ull;
   const uint32_t addr = smem_u32(bar);
   uint64_t start = 0;
   for (uint32_t i = 1;; ++i) {
@@ -282,7 +283,6 @@ __device__ __forceinline__ bool fp8_wait(uint64_t* bar, uint32_t parity, unsigne
         : "memory");
     if (done) return true;
     if ((i & 63u) == 0u) {
-      if (stop_on_error && error_raised()) return false;
       const uint64_t now = globaltimer_ns();
       if (start == 0) {
         start = now;
@@ -317,16 +317,19 @@ __device__ __forceinline__ TileEntry fp8_tile(const Fp8GemmParams& p, int m) {
 }
 
 // g / (1 + exp(-g)) * u for two columns, in place of the gates. One reciprocal
-// serves both: 1 / (d0 d1) times the other denominator. exp(-g) is held below
-// 2^58, so that the product stays finite; a gate below -40 then gives up to
-// 40 * 2^-58 = 1.4e-16 instead of less, which no E4M3 block can tell from 0
-// beside values above 1e-12. The approximations are within 2^-22 of the value,
+// serves both: 1 / (d0 d1) times the other denominator. Gates are held at -40
+// (NaN stays NaN), so that the product of the denominators stays finite; a gate
+// below gives -40 / (1 + exp(40)) = -1.7e-16 instead of a value between that and
+// 0, which no E4M3 block can tell from 0 beside values above 1e-12. The
+// approximations are within 2^-22 of the value,
 // far below the rounding to E4M3 that follows.
 __device__ __forceinline__ void swiglu_pair_f32(float& g0, float& g1, float u0, float u1) {
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(g0) : "f"(-40.0f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(g1) : "f"(-40.0f));
   const float2 t = mul2_rn(make_float2(g0, g1), make_float2(-1.4426950408889634f, -1.4426950408889634f));
   float e0, e1, r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(fminf(t.x, 58.0f)));
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(fminf(t.y, 58.0f)));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(t.x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(t.y));
   const float d0 = 1.0f + e0, d1 = 1.0f + e1;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d0 * d1));
   g0 *= r * d1 * u0;
@@ -402,6 +405,7 @@ __global__ void __launch_bounds__(Fp8Shape<BN>::THREADS, 1)
       uint8_t* const dst0 = lane == 0 ? sA : sB + (lane == 2 ? 16384 : 0);
       const uint32_t dst_step = lane == 0 ? S::A_BYTES : S::B_BYTES;
       uint32_t stage = 0, phase = 0;
+      int issued = 0;
       bool ok = true;
       for (int u = first; u < total && ok; u += step) {
         const int m = u / n_tiles, n = u - m * n_tiles;
@@ -416,12 +420,16 @@ __global__ void __launch_bounds__(Fp8Shape<BN>::THREADS, 1)
           if (lane == 0) mbar_arrive_expect_tx(&full[stage], S::STAGE_BYTES);
           __syncwarp();
           if (lane < kCopies) tma_load_2d(dst0 + stage * dst_step, map, &full[stage], kb * 128, row);
+          ++issued;
           if (++stage == S::STAGES) {
             stage = 0;
             phase ^= 1u;
           }
         }
       }
+      // no copy is in flight when the block ends, on the way out after a timeout either
+      for (int i = issued < S::STAGES ? 0 : issued - S::STAGES; i < issued; ++i)
+        fp8_wait(&full[i % S::STAGES], (i / S::STAGES) & 1, kErrTimeoutProducer);
     } else if (warp == 1) {
       // ---------------- MMA issuer ----------------
       constexpr uint32_t idesc = idesc_e4m3(128, BN);
@@ -452,7 +460,7 @@ __global__ void __launch_bounds__(Fp8Shape<BN>::THREADS, 1)
       // ---------------- relay: products complete -> epilogue ----------------
       uint32_t stage = 0, phase = 0;
       for (int i = 0; i < turns; ++i) {
-        fp8_wait(&done[stage], phase, kErrTimeoutEpilogue, 2000000000ull, false);
+        fp8_wait(&done[stage], phase, kErrTimeoutEpilogue);
         __syncwarp();
         named_sync(kFp8BarSums + i % S::BUFS, 32 * (S::EPI_WARPS + 1));
         if (++stage == S::STAGES) {

@@ -261,6 +261,8 @@ def test_linear_refuses_at_the_c_level(P):
                dict(k=0)):
         assert call(**kw) == P.capi.EINVAL, kw
     assert call() == P.capi.OK
+    # 2^24 x 2^7 tiles: their numbers would pass 31 bits (refused before anything is read)
+    assert call(rows=0x7fffff00, n=32768) == P.capi.EINVAL and b"tiles" in lib.praxis_b200_last_error()
     # up to 8 rows need no workspace
     assert lib.praxis_b200_fp8_linear_workspace_size(8, 128, 256) == 0
     with pytest.raises(ValueError):
@@ -281,6 +283,26 @@ def test_mlp(P, m, c, f):
     out = torch.full_like(x, 3.0)
     assert P.ops.fp8_mlp(x, *gu, *down, out=out) is out and same_bits(out, y)
     assert P.ops.fp8_mlp(x[:0], *gu, *down).shape == (0, c)
+
+
+@pytest.mark.parametrize("m", [3, 200])
+def test_mlp_of_closed_gates(P, m):
+    """silu lies between -40 / (1 + e^40) and 0 for gates below -40, and is
+    taken as that bound: |h| <= 1.7e-16 |u|, and an output at most the sum of
+    |h| |w|, with a rounding each to E4M3 and to bf16 (2^-4 and 2^-8)."""
+    c, f = 128, 256
+    one = torch.ones(c, dtype=BF16)
+    x = (one * 64.0).expand(m, c).contiguous().to(DEV)
+    gate_up = torch.cat([torch.full((f, c), -4.0), torch.full((f, c), 4.0)])  # gates -32768, up values 32768
+    gu = P.ops.fp8_pack_weights(gate_up.T.contiguous().to(BF16).to(DEV))
+    down = P.ops.fp8_pack_weights(torch.ones(f, c, dtype=BF16, device=DEV))
+    bound = 40 / (1 + math.exp(40)) * 32768 * f
+    y = P.ops.fp8_mlp(x, *gu, *down).double()
+    assert float(y.abs().max()) <= bound * (1 + 2**-4) * (1 + 2**-8)
+    # NaN stays in its row
+    x[1] = float("nan")
+    y2 = P.ops.fp8_mlp(x, *gu, *down).double()
+    assert bool(y2[1].isnan().all()) and torch.equal(y2[2], y[2])
 
 
 def routing(g, t, e, k, kind):
@@ -614,6 +636,7 @@ def test_two_captured_graphs_and_eager_calls(P, t):
 
 
 @pytest.mark.parametrize("t", [1, 70])
+@torch.no_grad()
 def test_captured_layer(P, t):
     """The graph pool finds layers with FP8 experts and replays their forward."""
     g = gen(80 + t)

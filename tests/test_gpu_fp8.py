@@ -492,6 +492,28 @@ def test_route_groups_ties_go_to_the_lower_index(P):
     assert torch.equal(idx, torch.arange(4, device=DEV).expand(3, 4)) and bool((gate == 0.25).all())
 
 
+@pytest.mark.parametrize("score", ["top2", "max"])
+@pytest.mark.parametrize("t,e,groups,top,k", ROUTES)
+def test_route_groups_many_ties(P, t, e, groups, top, k, score):
+    g = gen(t + e)
+    logits = torch.randint(0, 2, (t, e), generator=g).float().to(DEV)
+    idx, gate = P.ops.route(logits, None, k, "sigmoid", groups=groups, top_groups=top, group_score=score)
+    want, want_gate, _ = route64(logits, None, k, "sigmoid", groups, top, score)
+    assert torch.equal(idx, want)
+    assert bool(((gate.double() - want_gate).abs() <= 1.01 * 2**-8 * want_gate).all())
+
+
+@pytest.mark.parametrize("e,groups", [(256, 8), (64, 4), (130, 2)])
+def test_route_groups_unaligned_rows_and_bias(P, e, groups):
+    g = gen(e)
+    logits, bias = torch.randn(50, e, generator=g).to(DEV), torch.randn(e, generator=g).to(DEV)
+    run = lambda lo, bi: P.ops.route(lo, bi, 6, groups=groups, top_groups=2)  # noqa: E731
+    shift = lambda t: torch.cat([t.new_zeros(1), t.flatten()])[1:].view(t.shape)  # noqa: E731
+    want = run(logits, bias)
+    for other in (run(shift(logits), bias), run(logits, shift(bias)), run(shift(logits), shift(bias))):
+        assert torch.equal(other[0], want[0]) and same_bits(other[1], want[1])
+
+
 @pytest.mark.parametrize("act", ["sigmoid", "softmax"])
 def test_route_groups_masked_experts(P, act):
     """Masked experts (-inf) are picked last; a row with nothing left has

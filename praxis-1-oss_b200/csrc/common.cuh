@@ -41,7 +41,10 @@ __device__ __forceinline__ void record_error(unsigned int code) {
 // kernel's tail. pdl_wait(), the first statement of each such kernel, blocks
 // until the previous kernel has completed and its writes are visible (a no-op
 // for a kernel launched without the attribute); pdl_trigger() lets the next
-// kernel be scheduled once every CTA of this one has started.
+// kernel be scheduled once every CTA of this one has got there. It stands behind
+// pdl_wait() everywhere, so a kernel starts when all but the one before it has
+// completed; kernels that follow a known one of the same call may read what that
+// one does not write before they wait.
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

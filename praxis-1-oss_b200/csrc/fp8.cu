@@ -60,8 +60,11 @@ constexpr int kFp8QuantCols = 1024;  // per warp
 __global__ void __launch_bounds__(32 * kFp8QuantWarps, 6) fp8_quantize_kernel(
     const uint16_t* __restrict__ x, int64_t rows, int cols, int64_t ldx, Fp8Rows to, uint8_t* __restrict__ q,
     float* __restrict__ scale, int64_t scale_ld) {
-  pdl_wait();  // the previous kernel of the stream has completed
-  pdl_trigger();
+  // routed, the previous kernel is the dispatch, which writes no row of x
+  if (to.top_idx == nullptr) {
+    pdl_wait();
+    pdl_trigger();
+  }
   const int lane = threadIdx.x & 31;
   const int64_t row = (int64_t)blockIdx.x * kFp8QuantWarps + (threadIdx.x >> 5);
   if (row >= rows) return;
@@ -71,12 +74,6 @@ __global__ void __launch_bounds__(32 * kFp8QuantWarps, 6) fp8_quantize_kernel(
   for (int u = 0; u < 4; ++u) {
     v[u] = make_uint4(0u, 0u, 0u, 0u);
     if (col0 + 256 * u < cols) v[u] = ldg_stream(reinterpret_cast<const uint4*>(x + row * ldx + col0 + 256 * u));
-  }
-  int64_t dest = row;
-  if (to.top_idx != nullptr && lane < to.top_k) {
-    const int64_t p = row * to.top_k + lane;
-    const int e = checked_expert(to.top_idx[p], to.experts);
-    dest = (int64_t)to.pcsr[e] + to.inverse[p] - to.csr[e];
   }
   uint2 codes[4];
   float s[4];
@@ -92,6 +89,16 @@ __global__ void __launch_bounds__(32 * kFp8QuantWarps, 6) fp8_quantize_kernel(
     s[u] = div_rn(a, kE4m3Max);
     codes[u] = make_uint2(cvt_e4m3x4(mul_rn(f[0].x, r), mul_rn(f[0].y, r), mul_rn(f[1].x, r), mul_rn(f[1].y, r)),
                           cvt_e4m3x4(mul_rn(f[2].x, r), mul_rn(f[2].y, r), mul_rn(f[3].x, r), mul_rn(f[3].y, r)));
+  }
+  int64_t dest = row;
+  if (to.top_idx != nullptr) {
+    pdl_wait();
+    pdl_trigger();
+    if (lane < to.top_k) {
+      const int64_t p = row * to.top_k + lane;
+      const int e = checked_expert(to.top_idx[p], to.experts);
+      dest = (int64_t)to.pcsr[e] + to.inverse[p] - to.csr[e];
+    }
   }
   for (int j = 0; j < to.top_k; ++j) {
     const int64_t d = (int64_t)__shfl_sync(0xffffffffu, (unsigned long long)dest, j);
@@ -345,8 +352,6 @@ __device__ constexpr uint32_t chunk_col(int c) {
 template <int BN, int MODE>
 __global__ void __launch_bounds__(Fp8Shape<BN>::THREADS, 1)
     fp8_gemm_kernel(const __grid_constant__ Fp8GemmParams p) {
-  pdl_wait();  // the previous kernel of the stream has completed
-  pdl_trigger();
   using S = Fp8Shape<BN>;
   static_assert(MODE == FP8_PLAIN || BN == 256, "a SwiGLU tile is one block of 128 hidden columns");
   extern __shared__ uint8_t smem_raw[];
@@ -404,16 +409,46 @@ __global__ void __launch_bounds__(Fp8Shape<BN>::THREADS, 1)
       const CUtensorMap* map = lane == 0 ? &p.tmap_a : &p.tmap_b;
       uint8_t* const dst0 = lane == 0 ? sA : sB + (lane == 2 ? 16384 : 0);
       const uint32_t dst_step = lane == 0 ? S::A_BYTES : S::B_BYTES;
-      uint32_t stage = 0, phase = 0;
-      int issued = 0;
-      bool ok = true;
-      for (int u = first; u < total && ok; u += step) {
+      const int part = lane == 2 ? 1 : 0;  // weight rows of columns 0..127, 128..255
+      auto first_row = [&](int u) {
         const int m = u / n_tiles, n = u - m * n_tiles;
         const TileEntry t = fp8_tile(p, m);
-        const int part = lane == 2 ? 1 : 0;  // weight rows of columns 0..127, 128..255
-        const int row = lane == 0 ? t.row0
-                                  : t.expert * p.N + (MODE == FP8_SWIGLU ? n * 128 + part * F : n * BN + part * 128);
-        for (int kb = 0; kb < k_blocks; ++kb) {
+        return lane == 0 ? t.row0 : t.expert * p.N + (MODE == FP8_SWIGLU ? n * 128 + part * F : n * BN + part * 128);
+      };
+      // The weights and the table were there before the previous kernel began
+      // (see run_fp8_gemm): the first stages' weight rows come in while it ends,
+      // their A rows after it (64 x 1024 x 1024 in a row of calls 7.8 -> 7.0 us,
+      // 256 tokens through 4 of 64 experts 149 -> 145 us).
+      const int early = min(turns, S::STAGES);
+      int u = first, kb = 0, row = turns > 0 ? first_row(first) : 0;
+      auto next = [&] {
+        if (++kb == k_blocks) {
+          kb = 0;
+          u += step;
+          if (u < total) row = first_row(u);
+        }
+      };
+#pragma unroll 1
+      for (int s = 0; s < early; ++s, next()) {
+        if (lane == 0) mbar_arrive_expect_tx(&full[s], S::STAGE_BYTES);
+        __syncwarp();
+        if (lane > 0 && lane < kCopies) tma_load_2d(dst0 + s * dst_step, map, &full[s], kb * 128, row);
+      }
+      u = first;
+      kb = 0;
+      row = turns > 0 ? first_row(first) : 0;
+      pdl_wait();
+      pdl_trigger();
+#pragma unroll 1
+      for (int s = 0; s < early; ++s, next())
+        if (lane == 0) tma_load_2d(dst0 + s * dst_step, map, &full[s], kb * 128, row);
+      __syncwarp();
+      uint32_t stage = early % S::STAGES, phase = early / S::STAGES;
+      int issued = early;
+      bool ok = true;
+      for (; u < total && ok; u += step, kb = 0) {
+        row = first_row(u);
+        for (; kb < k_blocks; ++kb) {
           ok = fp8_wait(&done[stage], phase ^ 1u, kErrTimeoutProducer);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
@@ -428,6 +463,7 @@ __global__ void __launch_bounds__(Fp8Shape<BN>::THREADS, 1)
         }
       }
       // no copy is in flight when the block ends, on the way out after a timeout either
+#pragma unroll 1
       for (int i = issued < S::STAGES ? 0 : issued - S::STAGES; i < issued; ++i)
         fp8_wait(&full[i % S::STAGES], (i / S::STAGES) & 1, kErrTimeoutProducer);
     } else if (warp == 1) {
@@ -489,6 +525,7 @@ __global__ void __launch_bounds__(Fp8Shape<BN>::THREADS, 1)
   } else {
     if constexpr (S::SPLIT_REGS) regs_up<S::EPI_REGS>();
     // ---------------- epilogue ----------------
+    pdl_wait();
     const uint32_t quad = (uint32_t)(warp & 3);
     const int h = (warp - S::EPI_WARP0) >> 2;  // columns COLS h .. (SwiGLU: gate 64 h .. and up 128 + 64 h ..)
     const int row_in_tile = (int)(quad * 32 + lane);
@@ -773,8 +810,12 @@ __device__ __forceinline__ void mma_e4m3_16x8x32(float (&d)[4], uint32_t a0, uin
 template <int OP>
 __global__ void __launch_bounds__(32 * fp8_stream_warps<OP>(), 16 / fp8_stream_warps<OP>())
     fp8_stream_kernel(const __grid_constant__ Fp8StreamParams p) {
-  pdl_wait();  // the previous kernel of the stream has completed
-  pdl_trigger();
+  // behind UP, which writes the hidden rows alone, DOWN loads its first weights
+  // before it waits
+  if (OP != FP8_STREAM_DOWN) {
+    pdl_wait();
+    pdl_trigger();
+  }
   constexpr int WARPS = fp8_stream_warps<OP>();
   constexpr int SETS = OP == FP8_STREAM_UP ? 2 : 1;
   constexpr int AHEAD = 4 / SETS;  // k-blocks of a warp whose loads are in flight
@@ -834,6 +875,10 @@ __global__ void __launch_bounds__(32 * fp8_stream_warps<OP>(), 16 / fp8_stream_w
   };
 #pragma unroll
   for (int i = 0; i < AHEAD; ++i) load(i, blockIdx.x * 16, kb0 + i * step);
+  if (OP == FP8_STREAM_DOWN) {
+    pdl_wait();
+    pdl_trigger();
+  }
   const int pitch = fp8_stream_pitch(p.K);
   float* scales = reinterpret_cast<float*>(s_codes + (size_t)rows * pitch);
   fp8_stream_quantize<T, 32 * WARPS, OP == FP8_STREAM_UP ? 2 : 4>(x, p.ldx, rows, p.K, s_codes, scales);
@@ -980,7 +1025,10 @@ int run_fp8_pack(const uint16_t* w, int64_t experts, int64_t k, int64_t n, uint8
   return check_launch("fp8_pack");
 }
 
-// One GEMM over quantized rows. Dense (tiles == nullptr): `rows` rows against
+// One GEMM over quantized rows, launched behind the kernel that wrote them
+// (the quantization or the gate/up GEMM, which write neither the weights nor
+// the tile table and let this one start only when all before them is done).
+// Dense (tiles == nullptr): `rows` rows against
 // one weight. Grouped: the dispatch's tables, rows = padded rows, max_tiles
 // bounds the 128-row tiles. out (FP8_PLAIN) or hq / hs (FP8_SWIGLU) get the result.
 struct Fp8Gemm {

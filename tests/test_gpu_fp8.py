@@ -657,6 +657,47 @@ def test_two_captured_graphs_and_eager_calls(P, t):
             assert same_bits(got, w)
 
 
+@pytest.mark.parametrize("t", [1, 5, 48, 700])
+def test_calls_in_a_row_see_each_others_results(P, t):
+    """Inputs, routing and weights written by the call right before: the same
+    bits queued back to back, captured, and with a wait after every call."""
+    g = gen(90 + t)
+    c, f, e, k = 256, 384, 8, 2
+    banks = [(randn(g, e, c, 2 * f, scale=0.06), randn(g, e, f, c, scale=0.06)) for _ in range(3)]
+    square = randn(g, c, c, scale=0.06)
+    x0 = randn(g, t, c)
+    router = randn(g, e, c, dtype=torch.float32)
+    terms = P.ops.split_router_weight(router)
+
+    def chain(after=lambda: None):
+        x = x0
+        for gate_up, down in banks:
+            w = P.ops.fp8_pack_weights(square)
+            after()
+            x = P.ops.fp8_linear(x, *w)
+            after()
+            top, gate = P.ops.route(P.ops.router_logits(x, terms)[0], None, k, groups=4, top_groups=2)
+            after()
+            gu, dn = P.ops.fp8_pack_weights(gate_up), P.ops.fp8_pack_weights(down)
+            after()
+            x = x + P.ops.fp8_moe_forward(x, top, gate, *gu, *dn, 1.0)
+            after()
+            x = P.ops.fp8_mlp(x, *(q[0] for q in gu), *(q[0] for q in dn))
+            after()
+        return x
+
+    want = chain(torch.cuda.synchronize)
+    for _ in range(5):
+        assert same_bits(chain(), want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = chain()
+    for _ in range(5):
+        got.zero_()
+        graph.replay()
+        assert same_bits(got, want)
+
+
 @pytest.mark.parametrize("t", [1, 70])
 @torch.no_grad()
 def test_captured_layer(P, t):

@@ -230,7 +230,7 @@ static Fp8LinearLayout fp8_linear_layout(int64_t rows, int64_t k) {
 // The feed-forward: `rows` are the tokens (dense) or the padded routed rows.
 struct Fp8FfnLayout {
   size_t stream_hidden, stream_y, stream_inverse, stream_top, stream_gate, stream_csr, stream_pcsr;  // streaming path
-  size_t dispatch, inverse, csr, pcsr, offsets, tiles, num_tiles, aq, as, hq, hs, rows, total;
+  size_t slots, inverse, csr, pcsr, tiles, num_tiles, aq, as, hq, hs, rows, total;
   int64_t rp, scale_ld;
   int max_tiles;
 };
@@ -248,12 +248,11 @@ static Fp8FfnLayout fp8_ffn_layout(int64_t tokens, int top_k, int experts, int d
   L.rp = routed ? padded_rows(r, experts) : tokens;
   L.scale_ld = (L.rp + 31) / 32 * 32;
   L.max_tiles = routed ? (int)(L.rp / 128) : 0;
-  L.dispatch = take(routed ? dispatch_workspace_bytes(tokens, top_k, experts) : 0);
+  L.slots = take(routed ? fp8_slots_workspace(experts) : 0);
   L.inverse = take((size_t)r * 8);
   L.csr = take(routed ? (size_t)(experts + 1) * 4 : 0);
   L.pcsr = take(routed ? (size_t)(experts + 1) * 4 : 0);
-  L.offsets = take(routed ? (size_t)experts * 4 : 0);
-  L.tiles = take(routed ? (size_t)(2 * L.max_tiles + 1) * sizeof(TileEntry) : 0);
+  L.tiles = take((size_t)L.max_tiles * sizeof(TileEntry));
   L.num_tiles = take(8);
   L.aq = take((size_t)L.rp * dim);
   L.as = take((size_t)(dim / 128) * L.scale_ld * 4);
@@ -808,8 +807,8 @@ int praxis_b200_fp8_ffn(const praxis_b200_fp8_ffn_args* a) {
   const bool routed = a->top_k != 0;
   if (a->dim < 128 || a->hidden < 128 || a->dim % 128 || a->hidden % 128)
     return set_error(PRAXIS_B200_EINVAL, "fp8_ffn: C and F must be multiples of 128");
-  if (a->experts < 1 || (routed ? a->top_k < 0 || a->top_k > 8 || a->top_k > a->experts : a->experts != 1))
-    return set_error(PRAXIS_B200_EINVAL, "fp8_ffn: needs top_k 1..min(8, E), or one expert and no routing");
+  if (a->experts < 1 || a->experts > kFp8SlotThreads || (routed ? a->top_k < 0 || a->top_k > 8 || a->top_k > a->experts : a->experts != 1))
+    return set_error(PRAXIS_B200_EINVAL, "fp8_ffn: needs up to 1024 experts and top_k 1..min(8, E), or one expert and no routing");
   if (a->tokens < 0 || a->tokens * (int64_t)(routed ? a->top_k : 1) >= 0x7f000000ll)
     return set_error(PRAXIS_B200_EINVAL, "fp8_ffn: too many rows");
   const int top_k = a->top_k;
@@ -869,10 +868,8 @@ int praxis_b200_fp8_ffn(const praxis_b200_fp8_ffn_args* a) {
   uint16_t* rows = routed ? reinterpret_cast<uint16_t*>(ws + L.rows) : static_cast<uint16_t*>(a->out);
   Fp8Rows to = kFp8SameRows;
   if (routed) {
-    rc = run_dispatch(a->top_idx, static_cast<const uint16_t*>(a->gate), nullptr, a->tokens, top_k, a->experts,
-                      Passes{1, 0}, ws + L.dispatch, L.inverse - L.dispatch, nullptr, inverse, nullptr, nullptr,
-                      nullptr, reinterpret_cast<int32_t*>(ws + L.offsets), csr, pcsr, tiles, L.max_tiles, num_tiles,
-                      nullptr, nullptr, s);
+    rc = run_fp8_slots(a->top_idx, a->tokens * top_k, a->experts, ws + L.slots, inverse, csr, pcsr, tiles,
+                       L.max_tiles, num_tiles, s);
     if (rc) return rc;
     to = Fp8Rows{a->top_idx, inverse, csr, pcsr, top_k, a->experts};
   }

@@ -35,14 +35,107 @@ __device__ __forceinline__ uint32_t cvt_e4m3x4(float a, float b, float c, float 
 }
 
 // ---------------------------------------------------------------------------
+// Rows of the routed slots
+// ---------------------------------------------------------------------------
+// The experts' segments of rows, each padded to whole 128-row tiles, and a row
+// of its expert's segment for every routed slot p: pcsr[e] + inverse[p] - csr[e]
+// with csr = 0. Which row a slot gets within the segment depends on the order
+// of the CTAs; nothing else does, since every row is computed by itself and
+// read back through inverse. So one counting pass is enough (the dispatch of
+// the NVFP4 path keeps the slots' order: count, scan, scatter; 1024 slots of 32
+// experts 11 us there, 3.7 here, 65536 slots of 64 experts 32 and 14). A CTA takes
+// 4096 slots; with several of them each claims its share of every segment from
+// the counters, and the last one lays out the segments and their tiles.
+constexpr int kFp8SlotThreads = 1024;  // and the most experts
+constexpr int kFp8SlotItems = 4;
+
+__global__ void __launch_bounds__(kFp8SlotThreads) fp8_slots_kernel(
+    const int64_t* __restrict__ top_idx, int64_t positions, int experts, uint32_t* counters, int64_t* __restrict__ inverse,
+    int32_t* __restrict__ csr, int32_t* __restrict__ pcsr, TileEntry* __restrict__ tiles, int max_tiles,
+    int32_t* __restrict__ num_tiles) {
+  pdl_wait();  // the previous kernel of the stream has completed
+  pdl_trigger();
+  __shared__ uint32_t s_count[kFp8SlotThreads];  // slots per expert, then where this CTA's begin
+  __shared__ uint32_t s_warp[32];
+  __shared__ bool s_last;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  s_count[tid] = 0;
+  const int64_t p0 = (int64_t)blockIdx.x * (kFp8SlotThreads * kFp8SlotItems) + tid;
+  int e[kFp8SlotItems];
+  uint32_t rank[kFp8SlotItems];
+#pragma unroll
+  for (int i = 0; i < kFp8SlotItems; ++i) {
+    const int64_t p = p0 + i * kFp8SlotThreads;
+    e[i] = p < positions ? checked_expert(top_idx[p], experts) : -1;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kFp8SlotItems; ++i) {
+    const uint32_t peers = __match_any_sync(0xffffffffu, e[i]);
+    const int leader = __ffs(peers) - 1;
+    uint32_t before = 0;
+    if (lane == leader && e[i] >= 0) before = atomicAdd(&s_count[e[i]], (uint32_t)__popc(peers));
+    rank[i] = __shfl_sync(0xffffffffu, before, leader) + __popc(peers & ((1u << lane) - 1u));
+  }
+  __syncthreads();
+  const bool alone = gridDim.x == 1;
+  uint32_t count = s_count[tid], begin = 0;
+  if (!alone && count > 0) begin = atomicAdd(&counters[tid], count);
+  __syncthreads();
+  s_count[tid] = begin;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kFp8SlotItems; ++i)
+    if (e[i] >= 0) inverse[p0 + i * kFp8SlotThreads] = s_count[e[i]] + rank[i];
+  if (!alone) {
+    __threadfence();
+    __syncthreads();
+    if (tid == 0) s_last = atomicAdd(&counters[experts], 1u) == gridDim.x - 1;
+    __syncthreads();
+    if (!s_last) return;
+    __threadfence();
+    count = tid < experts ? __ldcg(&counters[tid]) : 0u;
+  }
+  // segments and tiles: an exclusive scan of the experts' tiles
+  const uint32_t mine = (count + kTileRows - 1) / kTileRows;
+  uint32_t sum = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t v = __shfl_up_sync(0xffffffffu, sum, o);
+    if (lane >= o) sum += v;
+  }
+  if (lane == 31) s_warp[warp] = sum;
+  __syncthreads();
+  uint32_t base = 0;
+  for (int w = 0; w < warp; ++w) base += s_warp[w];
+  const uint32_t end = base + sum, at = end - mine;
+  if (tid < experts) {
+    csr[tid] = 0;
+    pcsr[tid] = (int32_t)at * kTileRows;
+    if (tid == experts - 1) {
+      csr[experts] = 0;
+      pcsr[experts] = (int32_t)end * kTileRows;
+      num_tiles[0] = (int32_t)end;
+    }
+    for (uint32_t j = 0; j < mine && at + j < (uint32_t)max_tiles; ++j) {
+      TileEntry t;
+      t.expert = tid;
+      t.row0 = (int32_t)(at + j) * kTileRows;
+      t.valid = (int32_t)min(count - j * kTileRows, (uint32_t)kTileRows);
+      t.pad = 0;
+      tiles[at + j] = t;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
 // Activation quantization
 // ---------------------------------------------------------------------------
 // A warp takes 1024 columns of a row, four 16-byte loads per lane in flight;
 // sixteen lanes hold one block of 128 columns, whose largest magnitude is four
 // shuffles. Scales are stored block-major, scale[b * scale_ld + row]: the GEMM
 // epilogue reads one block's scales of 32 consecutive rows at once. With
-// `top_idx` the row goes to the rows of the token's routed slots (pcsr[e] +
-// inverse - csr[e], as the dispatch laid them out), quantized once.
+// `top_idx` the row goes to the rows of the token's routed slots, quantized once.
 struct Fp8Rows {
   const int64_t* top_idx;  // [rows, top_k]; nullptr: row r goes to row r
   const int64_t* inverse;
@@ -60,7 +153,7 @@ constexpr int kFp8QuantCols = 1024;  // per warp
 __global__ void __launch_bounds__(32 * kFp8QuantWarps, 6) fp8_quantize_kernel(
     const uint16_t* __restrict__ x, int64_t rows, int cols, int64_t ldx, Fp8Rows to, uint8_t* __restrict__ q,
     float* __restrict__ scale, int64_t scale_ld) {
-  // routed, the previous kernel is the dispatch, which writes no row of x
+  // routed, the previous kernel is fp8_slots_kernel, which writes no row of x
   if (to.top_idx == nullptr) {
     pdl_wait();
     pdl_trigger();
@@ -1007,6 +1100,22 @@ static int fp8_launch(const Fp8GemmParams& p, int64_t units, cudaStream_t stream
   return check_launch("fp8_gemm");
 }
 
+static size_t fp8_slots_workspace(int experts) { return (size_t)(experts + 1) * 4; }
+
+static int run_fp8_slots(const int64_t* top_idx, int64_t positions, int experts, void* workspace, int64_t* inverse,
+                         int32_t* csr, int32_t* pcsr, TileEntry* tiles, int max_tiles, int32_t* num_tiles,
+                         cudaStream_t stream) {
+  constexpr int64_t kPerCta = kFp8SlotThreads * kFp8SlotItems;
+  const int64_t ctas = (positions + kPerCta - 1) / kPerCta;
+  if (ctas > 1) {
+    const cudaError_t e = cudaMemsetAsync(workspace, 0, fp8_slots_workspace(experts), stream);
+    if (e != cudaSuccess) return set_error(PRAXIS_B200_ECUDA, "fp8 slots: %s", cudaGetErrorString(e));
+  }
+  launch_pdl(fp8_slots_kernel, dim3((unsigned)ctas), dim3(kFp8SlotThreads), 0, stream, top_idx, positions, experts,
+             static_cast<uint32_t*>(workspace), inverse, csr, pcsr, tiles, max_tiles, num_tiles);
+  return check_launch("fp8_slots");
+}
+
 int run_fp8_quantize(const uint16_t* x, int64_t rows, int cols, int64_t ldx, const Fp8Rows& to, uint8_t* q,
                      float* scale, int64_t scale_ld, cudaStream_t stream) {
   if (rows == 0) return PRAXIS_B200_OK;
@@ -1029,7 +1138,7 @@ int run_fp8_pack(const uint16_t* w, int64_t experts, int64_t k, int64_t n, uint8
 // (the quantization or the gate/up GEMM, which write neither the weights nor
 // the tile table and let this one start only when all before them is done).
 // Dense (tiles == nullptr): `rows` rows against
-// one weight. Grouped: the dispatch's tables, rows = padded rows, max_tiles
+// one weight. Grouped: fp8_slots_kernel's tables, rows = padded rows, max_tiles
 // bounds the 128-row tiles. out (FP8_PLAIN) or hq / hs (FP8_SWIGLU) get the result.
 struct Fp8Gemm {
   const uint8_t* q;
@@ -1111,7 +1220,7 @@ static int fp8_stream_launch(const Fp8StreamParams& p, int groups, cudaStream_t 
 // Whether a product of `rows` rows goes through the streaming kernels: dense up
 // to the 8 rows that share a weight; routed slots read their expert's weight
 // each for itself, so as long as they are few (C 2048, F 1536, 64 experts, cold
-// weights: 16 slots 48 us, through the dispatch and the tiles above 59; 32 slots
+// weights: 16 slots 48 us, through the tiles above 59; 32 slots
 // 75 against 86, 64 slots 134 against 113; 8 experts, C 1024, F 2048: 16 slots
 // 35 against 37, 24 slots 49 against 37). The quantized rows have to fit
 // the shared memory (k_up: columns of the rows, k_down: of the hidden rows, 0

@@ -320,7 +320,9 @@ EXPERTS = [(1, 256, 128, 8, 8, ""), (1, 512, 384, 64, 4, ""), (3, 128, 256, 8, 2
            (16, 384, 256, 16, 4, "skewed"), (33, 256, 384, 32, 6, ""), (40, 256, 256, 3, 2, "few"),
            (130, 256, 128, 5, 2, "skewed"), (257, 384, 256, 8, 3, ""), (900, 256, 384, 4, 2, ""),
            (1500, 128, 128, 2, 1, "skewed"), (700, 256, 256, 160, 8, ""),
-           (4000, 256, 512, 8, 2, "skewed")]
+           (4000, 256, 512, 8, 2, "skewed"), (2048, 128, 128, 4, 2, ""), (2049, 128, 128, 4, 2, "few"),
+           (9000, 128, 128, 1, 1, ""), (13000, 128, 128, 40, 5, "skewed"), (1, 128, 128, 1024, 8, ""),
+           (1500, 128, 128, 1024, 4, "")]
 
 
 @pytest.mark.parametrize("t,c,f,e,k,kind", EXPERTS)
@@ -338,6 +340,17 @@ def test_experts(P, t, c, f, e, k, kind):
     shared = randn(g, t, c)
     both = P.ops.fp8_moe_forward(x, top, gate, *gu, *down, 2.5, shared)
     assert torch.equal(both, (y.float() + shared.float()).to(BF16))
+
+
+@pytest.mark.parametrize("t", [1, 900])
+def test_more_than_1024_experts_are_refused(P, t):
+    c = f = 128
+    weights = [torch.zeros(1025, *s, device=DEV).to(d) for s, d in (((2 * f, c), F8), ((2, 1), torch.float32),
+                                                                   ((c, f), F8), ((1, 1), torch.float32))]
+    top = torch.zeros(t, 2, dtype=torch.int64, device=DEV)
+    with pytest.raises(Exception, match="1024 experts"):
+        P.ops.fp8_moe_forward(torch.zeros(t, c, dtype=BF16, device=DEV), top, torch.zeros(t, 2, dtype=BF16, device=DEV),
+                              *weights, 1.0)
 
 
 def test_experts_zero_tokens_zero_gates_and_special_rows(P):

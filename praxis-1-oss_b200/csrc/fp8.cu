@@ -1219,14 +1219,14 @@ static int fp8_stream_launch(const Fp8StreamParams& p, int groups, cudaStream_t 
 
 // Whether a product of `rows` rows goes through the streaming kernels: dense up
 // to the 8 rows that share a weight; routed slots read their expert's weight
-// each for itself, so as long as they are few (C 2048, F 1536, 64 experts, cold
-// weights: 16 slots 48 us, through the tiles above 59; 32 slots
-// 75 against 86, 64 slots 134 against 113; 8 experts, C 1024, F 2048: 16 slots
-// 35 against 37, 24 slots 49 against 37). The quantized rows have to fit
-// the shared memory (k_up: columns of the rows, k_down: of the hidden rows, 0
-// for a linear product).
+// each for itself, so as long as they are few, more of them where many experts
+// leave the tiles few rows each (streamed / in tiles, cold weights, us: C 2048,
+// F 1536, 64 experts, 16 slots 49 / 50, 24 slots 68 / 61; C 1024, F 2048, 8
+// experts, 8 slots 21 / 27, 12 slots 29 / 28; 32 experts, 12 slots 30 / 33, 16
+// slots 38 / 36). The quantized rows have to fit the shared memory (k_up:
+// columns of the rows, k_down: of the hidden rows, 0 for a linear product).
 static bool fp8_streams(int64_t rows, int top_k, int experts, int k_up, int k_down) {
-  if (top_k == 0 ? rows > 8 : rows * top_k > 16 && rows * top_k > experts / 2) return false;
+  if (top_k == 0 ? rows > 8 : rows * top_k > 8 + experts / 8) return false;
   return fp8_stream_smem(top_k == 0 ? (int)rows : 1, k_up) <= kFp8StreamSmemMax &&
          fp8_stream_smem(top_k == 0 ? (int)rows : top_k, k_down) <= kFp8StreamSmemMax;
 }

@@ -322,7 +322,8 @@ EXPERTS = [(1, 256, 128, 8, 8, ""), (1, 512, 384, 64, 4, ""), (3, 128, 256, 8, 2
            (1500, 128, 128, 2, 1, "skewed"), (700, 256, 256, 160, 8, ""),
            (4000, 256, 512, 8, 2, "skewed"), (2048, 128, 128, 4, 2, ""), (2049, 128, 128, 4, 2, "few"),
            (9000, 128, 128, 1, 1, ""), (13000, 128, 128, 40, 5, "skewed"), (1, 128, 128, 1024, 8, ""),
-           (1500, 128, 128, 1024, 4, "")]
+           (1500, 128, 128, 1024, 4, ""), (5, 256, 128, 16, 2, ""), (11, 256, 128, 16, 1, "few"),
+           (136, 128, 128, 1024, 1, ""), (137, 128, 128, 1024, 1, "")]
 
 
 @pytest.mark.parametrize("t,c,f,e,k,kind", EXPERTS)

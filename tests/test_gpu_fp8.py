@@ -671,7 +671,7 @@ def test_two_captured_graphs_and_eager_calls(P, t):
             assert same_bits(got, w)
 
 
-@pytest.mark.parametrize("t", [1, 5, 48, 700])
+@pytest.mark.parametrize("t", [1, 5, 48, 700, 2500])
 def test_calls_in_a_row_see_each_others_results(P, t):
     """Inputs, routing and weights written by the call right before: the same
     bits queued back to back, captured, and with a wait after every call."""

@@ -889,6 +889,7 @@ int praxis_b200_fp8_ffn(const praxis_b200_fp8_ffn_args* a) {
   g.tiles = routed ? tiles : nullptr;
   g.num_tiles = num_tiles;
   g.max_tiles = L.max_tiles;
+  g.slots = a->tokens * top_k;
   g.hq = ws + L.hq;
   g.hs = hs;
   g.hs_ld = L.scale_ld;

@@ -287,6 +287,7 @@ enum Fp8Mode : int { FP8_PLAIN = 0, FP8_SWIGLU = 1 };
 
 struct Fp8GemmParams {
   CUtensorMap tmap_a;    // activation codes [rows, K], boxes of 128 rows
+  CUtensorMap tmap_a32;  // the same, boxes of 32 rows (FEW)
   CUtensorMap tmap_b;    // weight codes [E * N, K], boxes of 128 rows
   CUtensorMap tmap_out;  // bf16 output [rows, N], boxes of 32 rows x 64 columns (tma_out)
   const float* xs;       // activation scales, [K blocks][xs_ld]
@@ -416,6 +417,11 @@ __device__ __forceinline__ TileEntry fp8_tile(const Fp8GemmParams& p, int m) {
   return t;
 }
 
+// A tile of up to 32 rows, loaded into all four quarters of the A operand: each
+// quadrant of tensor memory holds the sums of all its rows, and the warps of a
+// quadrant take a quarter of the columns instead of a quarter of the rows.
+constexpr int kFp8FewRows = 32;
+
 // g / (1 + exp(-g)) * u for two columns, in place of the gates. One reciprocal
 // serves both: 1 / (d0 d1) times the other denominator. Gates are held at -40
 // (NaN stays NaN), so that the product of the denominators stays finite; a gate
@@ -442,10 +448,11 @@ __device__ constexpr uint32_t chunk_col(int c) {
   return 16 * c + (MODE == FP8_SWIGLU && c >= 4 ? 64 : 0);
 }
 
-template <int BN, int MODE>
+template <int BN, int MODE, bool FEW>
 __global__ void __launch_bounds__(Fp8Shape<BN>::THREADS, 1)
     fp8_gemm_kernel(const __grid_constant__ Fp8GemmParams p) {
   using S = Fp8Shape<BN>;
+  static_assert(!FEW || BN == 256, "the few rows' columns are split for 256");
   static_assert(MODE == FP8_PLAIN || BN == 256, "a SwiGLU tile is one block of 128 hidden columns");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -499,14 +506,21 @@ __global__ void __launch_bounds__(Fp8Shape<BN>::THREADS, 1)
       // ---------------- TMA producer ----------------
       // one lane per copy: A, the weight rows, of 256 in two copies
       constexpr uint32_t kCopies = BN == 256 ? 3 : 2;
-      const CUtensorMap* map = lane == 0 ? &p.tmap_a : &p.tmap_b;
-      uint8_t* const dst0 = lane == 0 ? sA : sB + (lane == 2 ? 16384 : 0);
-      const uint32_t dst_step = lane == 0 ? S::A_BYTES : S::B_BYTES;
+      // (lanes 3..5: the second to fourth copy of up to 32 rows)
+      const bool b_lane = lane > 0 && lane < kCopies;
+      uint8_t* const dst0 = b_lane ? sB + (lane - 1) * 16384 : sA + (lane == 0 ? 0 : lane - 2) * 4096;
+      const uint32_t dst_step = b_lane ? S::B_BYTES : S::A_BYTES;
       const int part = lane == 2 ? 1 : 0;  // weight rows of columns 0..127, 128..255
+      const CUtensorMap* map = &p.tmap_b;
+      bool a_lane = false;
       auto first_row = [&](int u) {
         const int m = u / n_tiles, n = u - m * n_tiles;
         const TileEntry t = fp8_tile(p, m);
-        return lane == 0 ? t.row0 : t.expert * p.N + (MODE == FP8_SWIGLU ? n * 128 + part * F : n * BN + part * 128);
+        const bool few = FEW && t.valid <= kFp8FewRows;
+        a_lane = lane == 0 || (few && lane >= 3 && lane < 6);
+        if (!b_lane) map = few ? &p.tmap_a32 : &p.tmap_a;
+        return !b_lane ? t.row0
+                       : t.expert * p.N + (MODE == FP8_SWIGLU ? n * 128 + part * F : n * BN + part * 128);
       };
       // The weights and the table were there before the previous kernel began
       // (see run_fp8_gemm): the first stages' weight rows come in while it ends,
@@ -525,7 +539,7 @@ __global__ void __launch_bounds__(Fp8Shape<BN>::THREADS, 1)
       for (int s = 0; s < early; ++s, next()) {
         if (lane == 0) mbar_arrive_expect_tx(&full[s], S::STAGE_BYTES);
         __syncwarp();
-        if (lane > 0 && lane < kCopies) tma_load_2d(dst0 + s * dst_step, map, &full[s], kb * 128, row);
+        if (b_lane) tma_load_2d(dst0 + s * dst_step, map, &full[s], kb * 128, row);
       }
       u = first;
       kb = 0;
@@ -534,7 +548,7 @@ __global__ void __launch_bounds__(Fp8Shape<BN>::THREADS, 1)
       pdl_trigger();
 #pragma unroll 1
       for (int s = 0; s < early; ++s, next())
-        if (lane == 0) tma_load_2d(dst0 + s * dst_step, map, &full[s], kb * 128, row);
+        if (a_lane) tma_load_2d(dst0 + s * dst_step, map, &full[s], kb * 128, row);
       __syncwarp();
       uint32_t stage = early % S::STAGES, phase = early / S::STAGES;
       int issued = early;
@@ -547,7 +561,7 @@ __global__ void __launch_bounds__(Fp8Shape<BN>::THREADS, 1)
           if (!ok) break;
           if (lane == 0) mbar_arrive_expect_tx(&full[stage], S::STAGE_BYTES);
           __syncwarp();
-          if (lane < kCopies) tma_load_2d(dst0 + stage * dst_step, map, &full[stage], kb * 128, row);
+          if (a_lane || b_lane) tma_load_2d(dst0 + stage * dst_step, map, &full[stage], kb * 128, row);
           ++issued;
           if (++stage == S::STAGES) {
             stage = 0;
@@ -628,6 +642,7 @@ __global__ void __launch_bounds__(Fp8Shape<BN>::THREADS, 1)
     // two k-blocks, are fetched while the previous unit is written out.
     const int64_t up = MODE == FP8_SWIGLU ? (int64_t)(F / 128) * k_blocks : 0;
     int n = 0, valid = 0;
+    bool few = false;
     int64_t row = 0;
     const float *xs = nullptr, *ws = nullptr;
     float x0 = 0.0f, w00 = 0.0f, w01 = 0.0f, x1 = 0.0f, w10 = 0.0f, w11 = 0.0f;
@@ -636,7 +651,8 @@ __global__ void __launch_bounds__(Fp8Shape<BN>::THREADS, 1)
       const TileEntry t = fp8_tile(p, m);
       n = u - m * n_tiles;
       valid = t.valid;
-      row = (int64_t)t.row0 + row_in_tile;
+      few = FEW && valid <= kFp8FewRows;
+      row = (int64_t)t.row0 + (few ? (int)lane : row_in_tile);
       xs = p.xs + min(row, p.rows - 1);
       // the weight scales of this thread's columns: one row of blocks, or the
       // gate's and the up's
@@ -653,22 +669,90 @@ __global__ void __launch_bounds__(Fp8Shape<BN>::THREADS, 1)
     };
     uint32_t buf = 0, unit = 0;
     if (first < total) fetch(first);
+    // the scales of k-block kb, and the loads of those two blocks on
+    auto scales = [&](int kb, float& f0, float& f1) {
+      f0 = x0 * w00;
+      f1 = MODE == FP8_SWIGLU ? x0 * w01 : f0;
+      x0 = x1;
+      w00 = w10;
+      w01 = w11;
+      if (kb + 2 < k_blocks) {
+        x1 = __ldg(xs + (int64_t)(kb + 2) * p.xs_ld);
+        w10 = __ldg(ws + kb + 2);
+        if (MODE == FP8_SWIGLU) w11 = __ldg(ws + kb + 2 + up);
+      }
+    };
     for (int u = first; u < total; u += step, ++unit) {
+      uint32_t ra[16], rb[16];
+      if (FEW && few) {
+        // 32 columns: 32 in a row, or 16 of the gate and the same 16 of the up
+        float acc[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) acc[j] = 0.0f;
+        const uint32_t tf = tmem + ((quad * 32u) << 16) + (MODE == FP8_SWIGLU ? 64u * h + 16u * quad : 128u * h + 32u * quad);
+        for (int kb = 0; kb < k_blocks; ++kb) {
+          float f0, f1;
+          scales(kb, f0, f1);
+          named_sync(kFp8BarSums + buf, 32 * (S::EPI_WARPS + 1));
+          tc_fence_after();
+          tc_ld_32x32b_x16(tf + buf * BN, ra);
+          tc_ld_32x32b_x16(tf + buf * BN + (MODE == FP8_SWIGLU ? 128 : 16), rb);
+          tc_wait_ld();
+          tc_fence_before();
+          named_arrive(kFp8BarGo + buf, 32 * (S::EPI_WARPS + 2));
+          fp8_add_block(acc, ra, f0);
+          fp8_add_block(acc + 16, rb, f1);
+          if (++buf == S::BUFS) buf = 0;
+        }
+        const int n_out = n;
+        const int64_t row_out = row;
+        const bool live = (int)lane < valid;
+        if (u + step < total) fetch(u + step);
+        if constexpr (MODE == FP8_SWIGLU) {
+          float a = kFp8MinAmax;
+#pragma unroll
+          for (int j = 0; j < 16; j += 2) {
+            swiglu_pair_f32(acc[j], acc[j + 1], acc[16 + j], acc[17 + j]);
+            a = fmaxf(a, fmaxf(fabsf(acc[j]), fabsf(acc[j + 1])));
+          }
+          float* mx = s_max + (unit & 1u) * 256 + lane;
+          mx[(2 * quad + h) * 32] = a;
+          named_sync(kFp8BarMax, 32 * S::EPI_WARPS);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) a = fmaxf(a, mx[i * 32]);
+          if (live) {
+            const float r = div_rn(kE4m3Max, a);
+            uint32_t c[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              c[i] = cvt_e4m3x4(mul_rn(acc[4 * i], r), mul_rn(acc[4 * i + 1], r), mul_rn(acc[4 * i + 2], r),
+                                mul_rn(acc[4 * i + 3], r));
+            *reinterpret_cast<uint4*>(p.hq + row_out * F + n_out * 128 + 64 * h + 16 * quad) =
+                make_uint4(c[0], c[1], c[2], c[3]);
+            if (h == 0 && quad == 0) p.hs[(int64_t)n_out * p.hs_ld + row_out] = div_rn(a, kE4m3Max);
+          }
+        } else {
+          const int col = n_out * BN + 128 * h + 32 * (int)quad;
+          if (live && col < p.N) {
+            uint4* dst = reinterpret_cast<uint4*>(p.out + row_out * p.N + col);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float* v = acc + 8 * i;
+              dst[i] = make_uint4(cvt_bf16x2(v[0], v[1]), cvt_bf16x2(v[2], v[3]), cvt_bf16x2(v[4], v[5]),
+                                  cvt_bf16x2(v[6], v[7]));
+            }
+          }
+        }
+        __syncwarp();
+        continue;
+      }
       float acc[S::COLS];
 #pragma unroll
       for (int j = 0; j < S::COLS; ++j) acc[j] = 0.0f;
-      uint32_t ra[16], rb[16];
       for (int kb = 0; kb < k_blocks; ++kb) {
         const uint32_t tb = taddr + buf * BN;
-        const float f0 = x0 * w00, f1 = MODE == FP8_SWIGLU ? x0 * w01 : f0;
-        x0 = x1;
-        w00 = w10;
-        w01 = w11;
-        if (kb + 2 < k_blocks) {  // two blocks ahead of their use
-          x1 = __ldg(xs + (int64_t)(kb + 2) * p.xs_ld);
-          w10 = __ldg(ws + kb + 2);
-          if (MODE == FP8_SWIGLU) w11 = __ldg(ws + kb + 2 + up);
-        }
+        float f0, f1;
+        scales(kb, f0, f1);
         named_sync(kFp8BarSums + buf, 32 * (S::EPI_WARPS + 1));
         tc_fence_after();
         tc_ld_32x32b_x16(tb, ra);
@@ -1077,10 +1161,10 @@ static int fp8_map(CUtensorMap* map, CUtensorMapDataType type, int elem, const v
 }
 
 // Launches on at most one CTA per SM; `units` bounds the work.
-template <int BN, int MODE>
+template <int BN, int MODE, bool FEW>
 static int fp8_launch(const Fp8GemmParams& p, int64_t units, cudaStream_t stream) {
   using S = Fp8Shape<BN>;
-  auto kernel = fp8_gemm_kernel<BN, MODE>;
+  auto kernel = fp8_gemm_kernel<BN, MODE, FEW>;
   static DeviceOnce attr;
   const int rc = device_once(attr, [&](int dev) {
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM_BYTES);
@@ -1151,6 +1235,7 @@ struct Fp8Gemm {
   const TileEntry* tiles;
   const int32_t* num_tiles;
   int32_t max_tiles;
+  int64_t slots;  // routed rows without the padding
   uint16_t* out;
   uint8_t* hq;
   float* hs;
@@ -1176,6 +1261,15 @@ int run_fp8_gemm(const Fp8Gemm& g, cudaStream_t stream) {
     if (rc) return rc;
     p.tma_out = 1;
   }
+  // Few rows per tile on average: the kernel that splits such tiles by columns
+  // (4 of 64 experts, C 2048, F 1536, 64 tokens 136 -> 125 us, 512 tokens, 32 rows
+  // per expert, 139 -> 135; 1024 tokens 146 -> 149, so not beyond).
+  const bool few = !narrow && (swiglu || (p.tma_out && g.n % 32 == 0)) &&
+                   (g.tiles != nullptr ? g.slots <= (int64_t)kFp8FewRows * g.experts : g.rows <= kFp8FewRows);
+  if (few) {
+    rc = fp8_map(&p.tmap_a32, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, g.q, g.rows, g.k, kFp8FewRows);
+    if (rc) return rc;
+  }
   p.xs = g.xs;
   p.xs_ld = g.xs_ld;
   p.ws = g.ws;
@@ -1189,9 +1283,11 @@ int run_fp8_gemm(const Fp8Gemm& g, cudaStream_t stream) {
   p.hs = g.hs;
   p.hs_ld = g.hs_ld;
   p.tiles = g.tiles;
-  if (swiglu) return fp8_launch<256, FP8_SWIGLU>(p, m_tiles * n_tiles, stream);
-  if (narrow) return fp8_launch<64, FP8_PLAIN>(p, m_tiles * ((g.n + 63) / 64), stream);
-  return fp8_launch<256, FP8_PLAIN>(p, m_tiles * n_tiles, stream);
+  if (narrow) return fp8_launch<64, FP8_PLAIN, false>(p, m_tiles * ((g.n + 63) / 64), stream);
+  const int64_t units = m_tiles * n_tiles;
+  if (swiglu)
+    return few ? fp8_launch<256, FP8_SWIGLU, true>(p, units, stream) : fp8_launch<256, FP8_SWIGLU, false>(p, units, stream);
+  return few ? fp8_launch<256, FP8_PLAIN, true>(p, units, stream) : fp8_launch<256, FP8_PLAIN, false>(p, units, stream);
 }
 
 constexpr size_t kFp8StreamSmemMax = 160 * 1024;

@@ -323,7 +323,8 @@ EXPERTS = [(1, 256, 128, 8, 8, ""), (1, 512, 384, 64, 4, ""), (3, 128, 256, 8, 2
            (4000, 256, 512, 8, 2, "skewed"), (2048, 128, 128, 4, 2, ""), (2049, 128, 128, 4, 2, "few"),
            (9000, 128, 128, 1, 1, ""), (13000, 128, 128, 40, 5, "skewed"), (1, 128, 128, 1024, 8, ""),
            (1500, 128, 128, 1024, 4, ""), (5, 256, 128, 16, 2, ""), (11, 256, 128, 16, 1, "few"),
-           (136, 128, 128, 1024, 1, ""), (137, 128, 128, 1024, 1, "")]
+           (130, 256, 384, 32, 2, "skewed"), (200, 256, 128, 16, 2, "skewed"), (256, 128, 128, 8, 1, ""),
+           (257, 128, 128, 8, 1, ""), (136, 128, 128, 1024, 1, ""), (137, 128, 128, 1024, 1, "")]
 
 
 @pytest.mark.parametrize("t,c,f,e,k,kind", EXPERTS)
@@ -341,6 +342,20 @@ def test_experts(P, t, c, f, e, k, kind):
     shared = randn(g, t, c)
     both = P.ops.fp8_moe_forward(x, top, gate, *gu, *down, 2.5, shared)
     assert torch.equal(both, (y.float() + shared.float()).to(BF16))
+
+
+@pytest.mark.parametrize("t,c,f", [(40, 256, 128), (100, 640, 384), (128, 1024, 512)])
+def test_rows_do_not_depend_on_their_neighbours(P, t, c, f):
+    """The same bits in a small batch (few rows per tile) and in a large one."""
+    g = gen(t + c)
+    gu, down = weight(g, 4, 2 * f, c), weight(g, 4, c, f)
+    x = randn(g, 3000, c)
+    top, gate = routing(g, 3000, 4, 1, "")
+    whole = P.ops.fp8_moe_forward(x, top, gate, *gu, *down, 1.0)
+    part = P.ops.fp8_moe_forward(x[:t], top[:t], gate[:t], *gu, *down, 1.0)
+    assert same_bits(part, whole[:t])
+    dense = [q[0].contiguous() for q in (*gu, *down)]
+    assert same_bits(P.ops.fp8_mlp(x[:20], *dense), P.ops.fp8_mlp(x, *dense)[:20])
 
 
 @pytest.mark.parametrize("t", [1, 900])

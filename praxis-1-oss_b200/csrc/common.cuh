@@ -38,13 +38,21 @@ __device__ __forceinline__ void record_error(unsigned int code) {
 // Programmatic dependent launch. The hot-path kernels are launched with
 // launch_pdl (kernels.h): a kernel's CTAs may be scheduled while the previous
 // kernel of the stream is finishing, so its launch latency overlaps that
-// kernel's tail. pdl_wait(), the first statement of each such kernel, blocks
-// until the previous kernel has completed and its writes are visible (a no-op
-// for a kernel launched without the attribute); pdl_trigger() lets the next
-// kernel be scheduled once every CTA of this one has got there. It stands behind
-// pdl_wait() everywhere, so a kernel starts when all but the one before it has
-// completed; kernels that follow a known one of the same call may read what that
-// one does not write before they wait.
+// kernel's tail. pdl_wait() blocks until the previous kernel has completed and
+// its writes are visible (a no-op for a kernel launched without the attribute);
+// pdl_trigger() lets the next kernel be scheduled once every CTA of this one has
+// got there. It stands behind pdl_wait() everywhere, so a kernel starts when all
+// but the one before it has completed.
+//
+// pdl_wait() is the first statement of a kernel, except where the kernel follows
+// a known one of the same call: it may then read what that one does not write
+// before it waits (fp8.cu: the routed quantization, the GEMM's weights and tile
+// table, the streamed down product's weights and routing).
+//
+// What the previous kernel writes is written while this one is already there, so
+// it is not read-only for this kernel's lifetime: it is read with ordinary loads
+// behind pdl_wait(), not with __ldg, ld.global.nc or through a const __restrict__
+// parameter, which may be moved ahead of the wait and need not see the writes.
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
@@ -94,10 +102,11 @@ __device__ __forceinline__ uint32_t f32x2_to_e2m1_byte(float lo, float hi) {
   return out;
 }
 
-// 16-byte streaming load through the non-coherent path (read-once data).
+// 16-byte streaming load of read-once data. Not ld.global.nc: the callers read
+// results of the previous kernel with it too (see pdl_wait).
 __device__ __forceinline__ uint4 ldg_stream(const uint4* p) {
   uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
                : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                : "l"(p));
   return v;

@@ -50,7 +50,7 @@ constexpr int kFp8SlotThreads = 1024;  // and the most experts
 constexpr int kFp8SlotItems = 4;
 
 __global__ void __launch_bounds__(kFp8SlotThreads) fp8_slots_kernel(
-    const int64_t* __restrict__ top_idx, int64_t positions, int experts, uint32_t* counters, int64_t* __restrict__ inverse,
+    const int64_t* top_idx, int64_t positions, int experts, uint32_t* counters, int64_t* __restrict__ inverse,
     int32_t* __restrict__ csr, int32_t* __restrict__ pcsr, TileEntry* __restrict__ tiles, int max_tiles,
     int32_t* __restrict__ num_tiles) {
   pdl_wait();  // the previous kernel of the stream has completed
@@ -151,7 +151,7 @@ constexpr int kFp8QuantWarps = 8;
 constexpr int kFp8QuantCols = 1024;  // per warp
 
 __global__ void __launch_bounds__(32 * kFp8QuantWarps, 6) fp8_quantize_kernel(
-    const uint16_t* __restrict__ x, int64_t rows, int cols, int64_t ldx, Fp8Rows to, uint8_t* __restrict__ q,
+    const uint16_t* x, int64_t rows, int cols, int64_t ldx, Fp8Rows to, uint8_t* __restrict__ q,
     float* __restrict__ scale, int64_t scale_ld) {
   // routed, the previous kernel is fp8_slots_kernel, which writes no row of x
   if (to.top_idx == nullptr) {
@@ -639,7 +639,8 @@ __global__ void __launch_bounds__(Fp8Shape<BN>::THREADS, 1)
     const uint32_t taddr = tmem + ((quad * 32u) << 16) + (MODE == FP8_SWIGLU ? 64u : (uint32_t)S::COLS) * h;
     const int n_blocks = (p.N + kFp8Block - 1) / kFp8Block;
     // A unit's rows, columns and scale addresses, and the scales of its first
-    // two k-blocks, are fetched while the previous unit is written out.
+    // two k-blocks, are fetched while the previous unit is written out (the
+    // activation scales are the previous kernel's: ordinary loads).
     const int64_t up = MODE == FP8_SWIGLU ? (int64_t)(F / 128) * k_blocks : 0;
     int n = 0, valid = 0;
     bool few = false;
@@ -658,11 +659,11 @@ __global__ void __launch_bounds__(Fp8Shape<BN>::THREADS, 1)
       // gate's and the up's
       const int nb0 = MODE == FP8_SWIGLU ? n : min((n * BN + h * S::COLS) / kFp8Block, n_blocks - 1);
       ws = p.ws + ((int64_t)t.expert * n_blocks + nb0) * k_blocks;
-      x0 = __ldg(xs);
+      x0 = *xs;
       w00 = __ldg(ws);
       if (MODE == FP8_SWIGLU) w01 = __ldg(ws + up);
       if (k_blocks > 1) {
-        x1 = __ldg(xs + p.xs_ld);
+        x1 = xs[p.xs_ld];
         w10 = __ldg(ws + 1);
         if (MODE == FP8_SWIGLU) w11 = __ldg(ws + 1 + up);
       }
@@ -677,7 +678,7 @@ __global__ void __launch_bounds__(Fp8Shape<BN>::THREADS, 1)
       w00 = w10;
       w01 = w11;
       if (kb + 2 < k_blocks) {
-        x1 = __ldg(xs + (int64_t)(kb + 2) * p.xs_ld);
+        x1 = xs[(int64_t)(kb + 2) * p.xs_ld];
         w10 = __ldg(ws + kb + 2);
         if (MODE == FP8_SWIGLU) w11 = __ldg(ws + kb + 2 + up);
       }
@@ -913,9 +914,10 @@ __host__ __device__ constexpr size_t fp8_stream_smem(int rows, int k) {
   return (size_t)rows * (fp8_stream_pitch(k) + 4 * ((k + kFp8Block - 1) / kFp8Block));
 }
 
-// Eight activations of a row as floats.
+// Eight activations of a row as floats (the previous kernel's results, or may be:
+// ordinary loads).
 __device__ __forceinline__ void load8(const uint16_t* p, float (&v)[8]) {
-  const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
+  const uint4 u = *reinterpret_cast<const uint4*>(p);
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -927,7 +929,7 @@ __device__ __forceinline__ void load8(const uint16_t* p, float (&v)[8]) {
 __device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const float4 f = __ldg(reinterpret_cast<const float4*>(p) + i);
+    const float4 f = reinterpret_cast<const float4*>(p)[i];
     v[4 * i] = f.x;
     v[4 * i + 1] = f.y;
     v[4 * i + 2] = f.z;

@@ -34,7 +34,7 @@ __device__ __forceinline__ float rsqrt_hw(float v) {
 // Four consecutive bf16 (8 bytes) of a row, read once.
 __device__ __forceinline__ uint2 ldg_stream8(const uint16_t* p) {
   uint2 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  asm volatile("ld.global.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
   return v;
 }
 

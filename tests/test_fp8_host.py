@@ -3,6 +3,9 @@ without a GPU (fake CUDA tensors; nothing is launched)."""
 
 from __future__ import annotations
 
+import re
+from pathlib import Path
+
 import pytest
 import torch
 from conftest import pkg
@@ -198,3 +201,26 @@ def test_fake_shapes_of_the_torch_operators():
         assert torch.ops.praxis_b200.fp8_mlp(x, *weight(2 * f, c), *weight(c, f)).shape == (t, c)
         y = torch.ops.praxis_b200.fp8_moe_forward(x, top, gate, *weight(e, 2 * f, c), *weight(e, c, f), 2.5, None)
         assert (y.shape, y.dtype) == ((t, c), BF16)
+
+
+# -- kernels that overlap their predecessor --------------------------------------
+
+CSRC = Path(pkg().build.__file__).parent / "csrc"
+
+
+def code(name):
+    """A source file without its comments."""
+    return re.sub(r"//[^\n]*", "", (CSRC / name).read_text())
+
+
+def test_fp8_kernels_read_their_predecessors_results_with_ordinary_loads():
+    """A kernel that is launched before the previous one has ended may read what
+    that one writes with coherent loads only: read-only ones (__ldg, .nc, const
+    __restrict__ parameters) are for weights and their scales."""
+    fp8 = code("fp8.cu")
+    assert set(re.findall(r"__ldg\(\s*(\w+)", fp8)) <= {"ws"}
+    for name in ("common.cuh", "tail.cu", "fp8.cu"):
+        assert "ld.global.nc" not in code(name)
+    for kernel in ("fp8_slots_kernel", "fp8_quantize_kernel"):
+        params = re.search(kernel + r"\(([^)]*)\)\s*\{", fp8).group(1)
+        assert not re.search(r"const \w+\* __restrict__", params)

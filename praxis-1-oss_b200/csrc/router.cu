@@ -444,8 +444,8 @@ __device__ __forceinline__ void sort_descending(uint32_t (&v)[P]) {
 }
 
 template <int P>
-__global__ void __launch_bounds__(256) route_groups_kernel(const float* __restrict__ logits,
-                                                           const float* __restrict__ bias, int64_t tokens, int experts,
+__global__ void __launch_bounds__(256) route_groups_kernel(const float* logits, const float* bias,
+                                                           int64_t tokens, int experts,
                                                            int top_k, int activation, int groups, int top_groups,
                                                            int top2, int size, int per, int lpg_log2, int wide,
                                                            int wide_bias, int64_t* __restrict__ top_idx,
@@ -470,7 +470,7 @@ __global__ void __launch_bounds__(256) route_groups_kernel(const float* __restri
 #pragma unroll
     for (int i = 0; i < P; i += 4)
       if (i < mine) {
-        const float4 v = __ldg(reinterpret_cast<const float4*>(lr + i));
+        const float4 v = *reinterpret_cast<const float4*>(lr + i);
         score[i] = v.x;
         score[i + 1] = v.y;
         score[i + 2] = v.z;
@@ -509,7 +509,7 @@ __global__ void __launch_bounds__(256) route_groups_kernel(const float* __restri
 #pragma unroll
     for (int i = 0; i < P; i += 4)
       if (i < mine) {
-        const float4 v = __ldg(reinterpret_cast<const float4*>(bias + e0 + i));
+        const float4 v = *reinterpret_cast<const float4*>(bias + e0 + i);
         score[i] = add_rn(score[i], v.x);
         score[i + 1] = add_rn(score[i + 1], v.y);
         score[i + 2] = add_rn(score[i + 2], v.z);

@@ -224,3 +224,10 @@ def test_fp8_kernels_read_their_predecessors_results_with_ordinary_loads():
     for kernel in ("fp8_slots_kernel", "fp8_quantize_kernel"):
         params = re.search(kernel + r"\(([^)]*)\)\s*\{", fp8).group(1)
         assert not re.search(r"const \w+\* __restrict__", params)
+
+
+def test_grouped_router_reads_the_logits_with_ordinary_loads():
+    """The logits kernel is its predecessor."""
+    kernel = re.search(r"route_groups_kernel\(.*?\n}\n", code("router.cu"), re.S).group(0)
+    assert "__ldg" not in kernel
+    assert not re.search(r"const \w+\* __restrict__", kernel[: kernel.index("{")])

@@ -846,15 +846,19 @@ int praxis_b200_fp8_ffn(const praxis_b200_fp8_ffn_args* a) {
     p.shared = static_cast<const uint16_t*>(a->shared);
     p.hidden = reinterpret_cast<float*>(ws + L.stream_hidden);
     p.out = a->tail ? reinterpret_cast<uint16_t*>(ws + L.stream_y) : static_cast<uint16_t*>(a->out);
-    rc = run_fp8_stream_ffn(p, static_cast<const uint8_t*>(a->down_q), a->down_scale, a->dim, a->hidden, s);
-    if (rc || !a->tail) return rc;
     int64_t* inverse = reinterpret_cast<int64_t*>(ws + L.stream_inverse);
     int64_t* top_idx = reinterpret_cast<int64_t*>(ws + L.stream_top);
     uint16_t* gate = reinterpret_cast<uint16_t*>(ws + L.stream_gate);
     int32_t* csr = reinterpret_cast<int32_t*>(ws + L.stream_csr);
     int32_t* pcsr = reinterpret_cast<int32_t*>(ws + L.stream_pcsr);
-    rc = run_fp8_identity((int)a->tokens, inverse, top_idx, gate, csr, pcsr, s);
-    if (rc) return rc;
+    // before the products: the combine reads its dispatch as read-only data, so
+    // the kernel that writes it has to be over when the combine starts
+    if (a->tail) {
+      rc = run_fp8_identity((int)a->tokens, inverse, top_idx, gate, csr, pcsr, s);
+      if (rc) return rc;
+    }
+    rc = run_fp8_stream_ffn(p, static_cast<const uint8_t*>(a->down_q), a->down_scale, a->dim, a->hidden, s);
+    if (rc || !a->tail) return rc;
     return run_combine_tail(p.out, a->dim, inverse, top_idx, gate, csr, pcsr, nullptr, nullptr, nullptr, 1, 1.0f,
                             nullptr, tail_args(*a->tail), a->tokens, 1, 1, s);
   }

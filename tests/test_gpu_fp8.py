@@ -436,6 +436,39 @@ def test_bank_chunks_and_tail(P):
     assert normed is None and torch.equal(new, residual + both)
 
 
+@pytest.mark.parametrize("shared", [False, True])
+@pytest.mark.parametrize("kind", ["add", "norm", "mod", "mod_unfused", "mod_rows"])
+@pytest.mark.parametrize("t,chunk", [(1, 1), (3, 3), (5, 2), (52, 52), (300, 70)])
+def test_bank_tail_forms(P, t, chunk, kind, shared):
+    """Every form of the fused tail, behind the streaming and the tiled
+    products: the bits of the combine of the plain forward's output (one row per
+    token, gate 1), which has tests of its own."""
+    g = gen(t + 7 * len(kind))
+    c, f, e, k = 256, 128, 8, 2
+    gu, down = weight(g, e, 2 * f, c), weight(g, e, c, f)
+    bank = P.B200FP8RoutedExperts(dict(gate_up_q=gu[0], gate_up_scale=gu[1], down_q=down[0], down_scale=down[1]))
+    x, residual = randn(g, t, c), randn(g, t, c)
+    sh = randn(g, t, c) if shared else None
+    top, gate = routing(g, t, e, k, "")
+    tail = P.ops.Tail(residual)
+    if kind != "add":
+        tail = tail._replace(norm_weight=1 + randn(g, c, scale=0.1, dtype=torch.float32), eps=1e-6, norm_scale=0.8125)
+    if kind.startswith("mod"):
+        geom = (26, 8, 2, 2, 3, 2) if kind == "mod_rows" else None
+        rows = 8 * (-(-t // 26)) if geom else t
+        tail = tail._replace(mod=randn(g, rows, 2 * c, scale=0.2), mod_fma=kind != "mod_unfused", mod_geom=geom)
+    kw = dict(scaling=2.5, chunk_size=chunk)
+    y = (bank.routed_forward(x, top, gate, **kw) if sh is None
+         else bank.routed_forward_with_shared(x, top, gate, shared=sh, **kw))
+    same = P.ops.dispatch(torch.zeros(t, 1, dtype=torch.int64, device=DEV), torch.ones(t, 1, dtype=BF16, device=DEV), 1)
+    rows = torch.zeros(P.ops.padded_rows(t, 1), c, dtype=BF16, device=DEV)
+    rows[:t] = y
+    want = P.ops.combine_tail(rows, same, 1.0, tail, rows_rescaled=True)
+    new, normed = bank.routed_forward_tail(x, top, gate, tail=tail, shared=sh, **kw)
+    assert same_bits(new, want[0])
+    assert (normed is None and want[1] is None) if kind == "add" else same_bits(normed, want[1])
+
+
 def test_offsets_past_32_bits(P):
     """Weights of more than 2^32 bytes and activations of more than 2^32."""
     e, c, f = 65, 8192, 4096

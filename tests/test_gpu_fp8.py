@@ -188,6 +188,19 @@ def test_linear(P, m, n, k):
     assert same_bits(y, P.ops.fp8_linear(x, q, s))
 
 
+@pytest.mark.parametrize("m", [9, 17, 31, 32, 33])
+@pytest.mark.parametrize("n,k", [(9504, 128), (9728, 272), (9760, 1040), (9496, 256), (10001, 144)])
+def test_linear_few_rows_of_a_wide_weight(P, m, n, k):
+    """Up to 32 rows of a weight whose 256-column tiles fill the SMs: tiles of few
+    rows, split by columns (N a multiple of 32), and the forms beside them."""
+    g = gen(m + n + k)
+    q, s = weight(g, n, k)
+    x = randn(g, 64, k)
+    y = P.ops.fp8_linear(x[:m], q, s)
+    check_linear(y, x[:m], q, s)
+    assert same_bits(y, P.ops.fp8_linear(x, q, s)[:m])  # the rows of a larger batch: the wide form
+
+
 def test_linear_leading_dims_pitch_and_no_rows(P):
     g = gen(3)
     q, s = weight(g, 200, 256)

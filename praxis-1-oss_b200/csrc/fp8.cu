@@ -422,22 +422,23 @@ __device__ __forceinline__ TileEntry fp8_tile(const Fp8GemmParams& p, int m) {
 // quadrant take a quarter of the columns instead of a quarter of the rows.
 constexpr int kFp8FewRows = 32;
 
-// g / (1 + exp(-g)) * u for two columns, in place of the gates. One reciprocal
-// serves both: 1 / (d0 d1) times the other denominator. Gates are held at -40
-// (NaN stays NaN), so that the product of the denominators stays finite; a gate
-// below gives -40 / (1 + exp(40)) = -1.7e-16 instead of a value between that and
-// 0, which no E4M3 block can tell from 0 beside values above 1e-12. The
-// approximations are within 2^-22 of the value,
-// far below the rounding to E4M3 that follows.
+// g / (1 + exp(-g)) * u for two columns, in place of the gates. With
+// s = exp(-|g|), which lies in 0..1 and never overflows, the sigmoid is
+// 1 / (1 + s) for a gate above 0 and s / (1 + s) below, and one reciprocal
+// serves both columns: 1 / (d0 d1) times the other denominator, 1 <= d <= 2.
+// Relative error: 2^-22 of the approximations plus |g| 2^-24 of the rounded
+// exponent (2^-18 for a gate of -40), against the 2^-4 of the rounding to E4M3
+// that follows. exp(-|g|) below 2^-126 is 0: a gate below -87.3 gives 0 in place
+// of at most 1.1e-36 |u|. As the quotient has it, NaN stays NaN and a gate of
+// -inf gives NaN.
 __device__ __forceinline__ void swiglu_pair_f32(float& g0, float& g1, float u0, float u1) {
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(g0) : "f"(-40.0f));
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(g1) : "f"(-40.0f));
-  const float2 t = mul2_rn(make_float2(g0, g1), make_float2(-1.4426950408889634f, -1.4426950408889634f));
-  float e0, e1, r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(t.x));
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(t.y));
-  const float d0 = 1.0f + e0, d1 = 1.0f + e1;
+  float s0, s1, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(s0) : "f"(-1.4426950408889634f * fabsf(g0)));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(s1) : "f"(-1.4426950408889634f * fabsf(g1)));
+  const float d0 = 1.0f + s0, d1 = 1.0f + s1;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d0 * d1));
+  g0 *= g0 < 0.0f ? s0 : 1.0f;
+  g1 *= g1 < 0.0f ? s1 : 1.0f;
   g0 *= r * d1 * u0;
   g1 *= r * d0 * u1;
 }

@@ -318,6 +318,47 @@ def test_mlp_of_closed_gates(P, m):
     assert bool(y2[1].isnan().all()) and torch.equal(y2[2], y[2])
 
 
+@pytest.mark.parametrize("m", [3, 20, 200])
+def test_mlp_gates_far_below_zero(P, m):
+    """Every hidden column of a block has one gate value and u = 2^90, so the block
+    is held as 448 times its scale and an output is 128 h of its block. A gate of
+    C = 128 columns is off by (C + 4) 2^-23 of itself, which moves h = g e^g u by
+    that times |g|; the exponent's rounding and the approximations add
+    |g| 2^-24 + 2^-22, the block's scale and sum less than 2^-16, bf16 2^-8."""
+    c, values = 128, [-2.0, -39.0, -41.0, -45.0, -64.0, -80.0, -86.0, -120.0]
+    f = 128 * len(values)
+    x = torch.full((m, c), 64.0, dtype=BF16, device=DEV)
+    gate = torch.tensor(values).repeat_interleave(128)[:, None].expand(f, c) / (64 * c)
+    gate_up = torch.cat([gate, torch.full((f, c), 2.0**90 / (64 * c))])
+    gu = P.ops.fp8_pack_weights(gate_up.T.contiguous().to(BF16).to(DEV))
+    pick = torch.zeros(f, c)
+    for i in range(len(values)):
+        pick[128 * i:128 * (i + 1), 16 * i:16 * (i + 1)] = 1.0
+    down = P.ops.fp8_pack_weights(pick.to(BF16).to(DEV))
+    g64, u64 = (rows64(x) @ w64(*gu).T).chunk(2, dim=-1)
+    h64 = (g64 / (1 + torch.exp(-g64)) * u64)[:, ::128].repeat_interleave(16, 1) * 128
+    h64[:, 16 * 7:] = 0  # e^-120 is no 32-bit number
+    a = g64[:, ::128].repeat_interleave(16, 1).abs()
+    tol = (a * (c + 4) * 2.0**-23 + a * 2.0**-24 + 2.0**-22 + 2.0**-16) * 1.01 + 2.0**-8
+    y = P.ops.fp8_mlp(x, *gu, *down).double()
+    assert bool(((y - h64).abs() <= tol * h64.abs()).all()), ((y - h64) / h64)[0, ::16]
+
+
+@pytest.mark.parametrize("m", [3, 20, 200])
+def test_mlp_closed_and_overflowing_gates(P, m):
+    """Gates of -32768 leave exactly nothing; a gate that overflows to -inf gives
+    NaN in its row, as -inf times exp(-inf) does, and nowhere else."""
+    c, f = 128, 256
+    x = torch.full((m, c), 64.0, dtype=BF16, device=DEV)
+    gate_up = torch.cat([torch.full((f, c), -4.0), torch.full((f, c), 2.0**-20)])
+    gu = P.ops.fp8_pack_weights(gate_up.T.contiguous().to(BF16).to(DEV))
+    down = P.ops.fp8_pack_weights(torch.ones(f, c, dtype=BF16, device=DEV))
+    assert not P.ops.fp8_mlp(x, *gu, *down).any()
+    x[1] = 2.0**127
+    y = P.ops.fp8_mlp(x, *gu, *down)
+    assert bool(y[1].isnan().all()) and not y[[0, 2]].any()
+
+
 def routing(g, t, e, k, kind):
     logits = torch.randn(t, e, generator=g)
     if kind == "skewed":

@@ -777,11 +777,12 @@ def fp8_quantize(x: Tensor) -> tuple[Tensor, Tensor]:
     """The activation quantization of the FP8 products: (q E4M3 [R, K],
     scale fp32 [R, ceil(K / 128)]) of bf16 rows x [R, K], K % 16 == 0. A block
     of 128 columns with largest magnitude a = max(|x|, 1e-12) is held as
-    e4m3(x * f32(448 / a)) with scale f32(a / 448)."""
+    e4m3(x * f32(448 / a)) with scale f32(a / 448). Inference only."""
     if not isinstance(x, Tensor) or x.ndim != 2:
         raise ValueError("x: expected 2 dims")
     k = x.shape[1]
     x, r, pitch = _fp8_rows(x, k)
+    _inference_only(x)
     ld = -(-max(r, 1) // 32) * 32
     q = torch.empty(r, k, dtype=F8, device=x.device)
     scale = torch.empty(-(-k // 128), ld, dtype=torch.float32, device=x.device)
@@ -794,10 +795,13 @@ def fp8_quantize(x: Tensor) -> tuple[Tensor, Tensor]:
 def fp8_pack_weights(w: Tensor) -> tuple[Tensor, Tensor]:
     """Expert-first bf16 bank [E, K, N] (or one matrix [K, N]), input features
     first -> (q E4M3 [.., N, K], scale fp32 [.., ceil(N/128), ceil(K/128)])
-    on the GPU, the recipe of :func:`fp8_quantize` per 128 x 128 block."""
+    on the GPU, the recipe of :func:`fp8_quantize` per 128 x 128 block. The
+    packed weight carries no gradient: detach a parameter first, or call this
+    under ``torch.no_grad()``."""
     if not isinstance(w, Tensor) or w.ndim not in (2, 3):
         raise ValueError("weights: expected [E, K, N] or [K, N]")
     _need(w, "weights", BF16)
+    _inference_only(w)
     e = w.shape[0] if w.ndim == 3 else 1
     k, n = w.shape[-2:]
     q = torch.empty(w.shape[:-2] + (n, k), dtype=F8, device=w.device)
@@ -914,6 +918,7 @@ def fp8_moe_forward(x: Tensor, top_idx: Tensor, gate: Tensor, gate_up_q: Tensor,
     weights = (gate_up_q, gate_up_scale, down_q, down_scale)
     _inference_only(x, gate, shared, *weights)
     if tail is not None:
+        _inference_only(tail.residual, tail.norm_weight, tail.mod)
         st, residual_out, normed = _tail_struct(tail, t, c, x.device, tail_out)
         _fp8_ffn(x, t, top_idx, gate, shared, None, weights, sizes, float(scaling), st)
         return residual_out, normed

@@ -81,6 +81,27 @@ def test_products_refuse_gradients():
             pkg().ops.fp8_linear(cuda(4, 256), q, s.requires_grad_())
 
 
+@pytest.mark.parametrize("which", ["residual", "norm_weight", "mod", "shared"])
+def test_tail_refuses_gradients(which):
+    """The fused tail's outputs carry no gradient, so no input of it may want one."""
+    with FakeTensorMode():
+        e, c, f, t, k = 4, 256, 128, 6, 2
+        given = dict(residual=cuda(t, c), norm_weight=cuda(c, dtype=torch.float32), mod=cuda(t, 2 * c), shared=cuda(t, c))
+        given[which].requires_grad_()
+        shared = given.pop("shared")
+        with pytest.raises(RuntimeError, match="inference"):
+            pkg().ops.fp8_moe_forward(cuda(t, c), cuda(t, k, dtype=torch.int64), cuda(t, k), *weight(e, 2 * f, c),
+                                      *weight(e, c, f), 1.0, shared, tail=pkg().ops.Tail(**given))
+
+
+def test_quantizers_refuse_gradients():
+    with FakeTensorMode():
+        with pytest.raises(RuntimeError, match="inference"):
+            pkg().ops.fp8_quantize(cuda(4, 256).requires_grad_())
+        with pytest.raises(RuntimeError, match="inference"):
+            pkg().ops.fp8_pack_weights(cuda(256, 128).requires_grad_())
+
+
 @pytest.mark.parametrize("kind", ["odd", "small", "down", "out", "x_strided", "experts"])
 def test_mlp_refuses(kind):
     with FakeTensorMode():

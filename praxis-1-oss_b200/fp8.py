@@ -132,6 +132,9 @@ class B200FP8RoutedExperts(_FP8Experts):
             raise ValueError("FP8 inference requires a positive dispatch chunk size")
         if isinstance(scaling, bool) or not isinstance(scaling, float | int) or not math.isfinite(scaling):
             raise ValueError("Routed scaling must be finite")
+        # once for the whole call: a chunk's slices would hide rows of a longer tensor
+        if x.ndim != 2 or top_idx.ndim != 2 or top_idx.shape[0] != x.shape[0] or gate.shape != top_idx.shape:
+            raise ValueError("Expected routed activations [T, C] with expert indices and gates [T, k]")
 
     def _routed_forward(self, x: Tensor, top_idx: Tensor, gate: Tensor, *, scaling: float, chunk_size: int,
                         shared: Tensor | None = None) -> Tensor:
@@ -151,6 +154,8 @@ class B200FP8RoutedExperts(_FP8Experts):
         self._check(x, top_idx, gate, scaling, chunk_size)
         if tail.residual.shape != x.shape:
             raise ValueError("Expected a contiguous BF16 residual shaped like the routed activations")
+        if shared is not None and (shared.shape != x.shape or shared.dtype != x.dtype or not shared.is_contiguous()):
+            raise ValueError("Expected a contiguous BF16 shared-expert output shaped like the activations")
         residual_out = torch.empty_like(x)
         normed = None if tail.norm_weight is None else torch.empty_like(x)
         for start in range(0, x.shape[0], chunk_size):

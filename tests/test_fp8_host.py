@@ -196,6 +196,41 @@ def test_bank_is_inference_only_and_keeps_its_types():
     assert (again.num_experts, again.in_features, again.hidden_features) == (2, 128, 128)
 
 
+@pytest.mark.parametrize("kind,tail", [
+    *((kind, tail) for kind in ("top_more", "top_fewer", "gate_more", "gate_k", "x_3d") for tail in (False, True)),
+    ("shared", True), ("shared_dtype", True),  # without a tail such a shared output is added by torch
+])
+def test_bank_checks_the_whole_call_before_it_is_cut_in_chunks(monkeypatch, kind, tail):
+    """Rows behind the last token's must not vanish in the slices of the chunks."""
+    called = []
+    monkeypatch.setattr(pkg().ops, "fp8_moe_forward", lambda *a, **kw: called.append(1))
+    bank = pkg().B200FP8RoutedExperts.from_packed(packed())
+    t = 5
+    x, shared, residual = (torch.ones(t, 128, dtype=BF16) for _ in range(3))
+    top, gate = torch.zeros(t, 2, dtype=torch.int64), torch.ones(t, 2, dtype=BF16)
+    if kind == "shared":
+        shared = torch.ones(t + 3, 128, dtype=BF16)
+    elif kind == "shared_dtype":
+        shared = shared.float()
+    elif kind == "top_more":
+        top = torch.zeros(t + 3, 2, dtype=torch.int64)
+    elif kind == "top_fewer":
+        top, gate = top[:4], gate[:4]
+    elif kind == "gate_more":
+        gate = torch.ones(t + 3, 2, dtype=BF16)
+    elif kind == "gate_k":
+        gate = gate[:, :1]
+    else:
+        x = residual = torch.ones(t, 1, 128, dtype=BF16)
+    with pytest.raises(ValueError):
+        if tail:
+            bank.routed_forward_tail(x, top, gate, scaling=1.0, chunk_size=2, tail=pkg().ops.Tail(residual),
+                                     shared=shared)
+        else:
+            bank.routed_forward(x, top, gate, scaling=1.0, chunk_size=2)
+    assert not called
+
+
 def test_module_takes_groups_and_formats():
     M = pkg().B200MoEFeedForward
     m = M(128, 128, 16, 4, router_groups=4, router_top_groups=2)

@@ -476,7 +476,9 @@ typedef struct praxis_b200_fp8_ffn_args {
   const praxis_b200_tail* tail;
 } praxis_b200_fp8_ffn_args;
 
-/* top_k = 0: dense. */
+/* top_k = 0: dense. Grows with the rows (routed: with their tiles of 128, at
+ * most one partly filled per expert that has any), not with the experts; few
+ * rows, which are streamed, need a few KB each, and no tokens nothing. */
 size_t praxis_b200_fp8_ffn_workspace_size(int64_t tokens, int32_t top_k, int32_t experts, int32_t dim, int32_t hidden);
 int praxis_b200_fp8_ffn(const praxis_b200_fp8_ffn_args* args);
 

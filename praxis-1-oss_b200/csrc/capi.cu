@@ -245,7 +245,8 @@ static Fp8FfnLayout fp8_ffn_layout(int64_t tokens, int top_k, int experts, int d
   };
   const bool routed = top_k > 0;
   const int64_t r = tokens * top_k;
-  L.rp = routed ? padded_rows(r, experts) : tokens;
+  // experts without a slot have no rows
+  L.rp = routed ? padded_rows(r, r < experts ? r : experts) : tokens;
   L.scale_ld = (L.rp + 31) / 32 * 32;
   L.max_tiles = routed ? (int)(L.rp / 128) : 0;
   L.slots = take(routed ? fp8_slots_workspace(experts) : 0);
@@ -260,8 +261,8 @@ static Fp8FfnLayout fp8_ffn_layout(int64_t tokens, int top_k, int experts, int d
   L.hs = take((size_t)(hidden / 128) * L.scale_ld * 4);
   L.rows = take(routed ? (size_t)L.rp * dim * 2 : 0);
   L.total = off;
-  // The streaming path uses the same bytes: its fp32 hidden rows, and for a
-  // fused tail its output and a dispatch of the tokens to themselves.
+  // The streaming path has none of these: its fp32 hidden rows, and for a fused
+  // tail its output and a dispatch of the tokens to themselves.
   off = 0;
   L.stream_hidden = take((size_t)tokens * (routed ? top_k : 1) * hidden * 4);
   L.stream_y = take((size_t)tokens * dim * 2);
@@ -270,7 +271,8 @@ static Fp8FfnLayout fp8_ffn_layout(int64_t tokens, int top_k, int experts, int d
   L.stream_gate = take((size_t)tokens * 2);
   L.stream_csr = take(8);
   L.stream_pcsr = take(8);
-  if (fp8_streams(tokens, top_k, experts, dim, hidden) && off > L.total) L.total = off;
+  if (fp8_streams(tokens, top_k, experts, dim, hidden)) L.total = off;
+  if (tokens == 0) L.total = 0;
   return L;
 }
 

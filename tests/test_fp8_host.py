@@ -295,3 +295,29 @@ def test_the_streamed_tails_dispatch_is_complete_before_its_combine_starts():
     ffn = code("capi.cu")
     ffn = ffn[ffn.index("int praxis_b200_fp8_ffn("):]
     assert ffn.index("run_fp8_identity(") < ffn.index("run_fp8_stream_ffn(") < ffn.index("run_combine_tail(")
+
+
+# -- workspaces --------------------------------------------------------------------
+
+def ffn_workspace(tokens, top_k, experts, dim, hidden):
+    p = pkg()
+    p.build.build()
+    return p.capi.load().praxis_b200_fp8_ffn_workspace_size(tokens, top_k, experts, dim, hidden)
+
+
+@pytest.mark.parametrize("tokens", [1, 2, 6, 40, 1000])
+def test_workspace_follows_the_routed_slots_and_not_the_experts(tokens):
+    """At most min(E, slots) experts have rows, each padded by fewer than a tile."""
+    c, f, e, k = 7168, 2048, 256, 8
+    slots = tokens * k
+    rows = (slots + 127 * min(e, slots)) // 128 * 128
+    per_row = c + c // 128 * 4 + f + f // 128 * 4 + 2 * c  # codes and scales twice, the down rows in bf16
+    size = ffn_workspace(tokens, k, e, c, f)
+    assert size <= rows * per_row + slots * 8 + rows // 128 * 16 + 4 * (e + 1) * 3 + 32 * 4 * (c + f) // 128 + 4096
+    if slots <= 8 + e // 8:  # streamed: fp32 hidden rows, and what a fused tail needs
+        assert size <= slots * f * 4 + tokens * (c * 2 + 18) + 16 + 7 * 256
+
+
+def test_workspace_of_no_tokens_is_empty():
+    assert ffn_workspace(0, 8, 256, 7168, 2048) == 0
+    assert ffn_workspace(0, 0, 1, 1024, 512) == 0

@@ -851,3 +851,29 @@ def test_torch_operators_match_direct_calls(P):
     for op, args in ((ns.fp8_linear, (x, *lin)), (ns.fp8_mlp, (x, *dense)),
                      (ns.fp8_moe_forward, (x, top, gate, *gu, *down, 2.5, None))):
         torch.library.opcheck(op.default, args, test_utils=("test_faketensor",))
+
+
+@pytest.mark.parametrize("t,e,k", [(9, 160, 4), (40, 1024, 2), (1, 1024, 8), (150, 1024, 1), (17, 96, 8)])
+def test_few_slots_of_many_experts_stay_inside_their_workspace(P, t, e, k):
+    """Slots all on different experts (as far as they go): the most tiles that a
+    call can have. Nothing behind the workspace's stated size is written."""
+    g = gen(t + e)
+    c, f = 256, 128
+    gu, down = weight(g, e, 2 * f, c), weight(g, e, c, f)
+    x = randn(g, t, c)
+    top = (torch.arange(t * k).view(t, k) * 7 % e).to(DEV)
+    gate = randn(g, t, k).abs()
+    lib = P.capi.load()
+    size = lib.praxis_b200_fp8_ffn_workspace_size(t, k, e, c, f)
+    ws = torch.full((size + 4096,), 0xA5, dtype=torch.uint8, device=DEV)
+    out = torch.empty_like(x)
+    args = P.capi.Fp8FfnArgs(
+        x=x.data_ptr(), top_idx=top.data_ptr(), gate=gate.data_ptr(), out=out.data_ptr(), gate_up_q=gu[0].data_ptr(),
+        gate_up_scale=gu[1].data_ptr(), down_q=down[0].data_ptr(), down_scale=down[1].data_ptr(), tokens=t, dim=c,
+        hidden=f, experts=e, top_k=k, scaling=1.0, workspace=ws.data_ptr(), workspace_size=size, device=0,
+        stream=torch.cuda.current_stream().cuda_stream)
+    P.capi.check(lib.praxis_b200_fp8_ffn(args))
+    assert bool((ws[size:] == 0xA5).all())
+    want = experts64(rows64(x), top, gate, w64(*gu), w64(*down), 1.0)
+    assert rel(out, want) < 1e-2
+    assert same_bits(out, P.ops.fp8_moe_forward(x, top, gate, *gu, *down, 1.0))

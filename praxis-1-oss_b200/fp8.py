@@ -23,6 +23,13 @@ from . import ops
 _ROUTED_NAMES = frozenset(("gate_up_q", "gate_up_scale", "down_q", "down_scale"))
 
 
+def _any_nan(codes: Tensor) -> bool:
+    """Whether E4M3 codes hold a NaN; in pieces of 16 MB, since a bank may fill
+    most of its device."""
+    pieces = codes.view(torch.uint8).flatten().split(2**24)
+    return bool(torch.stack([((piece & 0x7F) == 0x7F).any() for piece in pieces]).any())
+
+
 def _validate(state: Mapping[str, Tensor], ndim: int) -> tuple[int, int, int]:
     """(E, C, F) of a gate/up and a down weight [.., 2F, C] and [.., C, F]."""
     if not isinstance(state, Mapping) or set(state) != _ROUTED_NAMES:
@@ -49,7 +56,7 @@ def _validate(state: Mapping[str, Tensor], ndim: int) -> tuple[int, int, int]:
             raise ValueError(f"Invalid FP8 buffer shape/dtype: {name}")
         if name.endswith("_scale") and not (torch.isfinite(value) & (value > 0)).all().item():
             raise ValueError(f"Invalid positive block scales: {name}")
-        if name.endswith("_q") and ((value.view(torch.uint8) & 0x7F) == 0x7F).any().item():
+        if name.endswith("_q") and _any_nan(value):
             raise ValueError(f"Invalid E4M3 values: {name}")
     return (lead[0] if lead else 1), c, f
 

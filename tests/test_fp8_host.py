@@ -10,6 +10,7 @@ import pytest
 import torch
 from conftest import pkg
 from torch._subclasses.fake_tensor import FakeTensorMode
+from torch.utils._python_dispatch import TorchDispatchMode
 
 BF16 = torch.bfloat16
 F8 = torch.float8_e4m3fn
@@ -173,6 +174,28 @@ def test_bank_rejects_corrupt_state(kind):
     else:
         state = packed(c=192)
     with pytest.raises(ValueError):
+        pkg().B200FP8RoutedExperts.from_packed(state)
+
+
+def test_bank_validation_needs_no_copies_of_the_bank():
+    """The search for NaN codes goes through the bank in pieces, and finds one in
+    the last of them."""
+    class Largest(TorchDispatchMode):
+        nbytes = 0
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            out = func(*args, **(kwargs or {}))
+            given = {a.untyped_storage().data_ptr() for a in args if isinstance(a, torch.Tensor)}
+            if isinstance(out, torch.Tensor) and out.untyped_storage().data_ptr() not in given:
+                self.nbytes = max(self.nbytes, out.nbytes)
+            return out
+
+    state = packed(e=3, c=4096, f=4096)
+    with Largest() as largest:
+        pkg().B200FP8RoutedExperts.from_packed(state)
+    assert largest.nbytes <= 2**24 < state["gate_up_q"].nbytes // 4
+    state["gate_up_q"].view(torch.uint8)[-1, -1, -1] = 0x7F
+    with pytest.raises(ValueError, match="E4M3"):
         pkg().B200FP8RoutedExperts.from_packed(state)
 
 

@@ -30,7 +30,7 @@ constexpr int kMaxExperts = 1024;
 // ---------------------------------------------------------------------------
 // Row max |x| (bf16), praxis/kernels/nvfp4_moe.py:15-21
 // ---------------------------------------------------------------------------
-__global__ void row_amax_kernel(const uint16_t* __restrict__ x, int64_t rows, int cols, uint16_t* __restrict__ out) {
+__global__ void row_amax_kernel(const uint16_t* x, int64_t rows, int cols, uint16_t* __restrict__ out) {
   pdl_wait();  // the previous kernel of the stream has completed
   pdl_trigger();
   const int warps = blockDim.x >> 5;
@@ -40,7 +40,7 @@ __global__ void row_amax_kernel(const uint16_t* __restrict__ x, int64_t rows, in
   const uint4* src = reinterpret_cast<const uint4*>(x + row * cols);
   float m = 0.0f;
   for (int i = lane; i < cols / 8; i += 32) {
-    uint4 v = __ldg(src + i);
+    uint4 v = src[i];
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -66,8 +66,8 @@ __device__ __forceinline__ int64_t token_of(int64_t p, int top_k) {
 // histogram bins (route_group).
 // One warp's segment: its per-group histogram h and max row-amax hm (this
 // warp's zeroed shared rows), then written to seg_count / seg_max.
-__device__ __forceinline__ void count_segment(const int64_t* __restrict__ top_idx,
-                                              const uint16_t* __restrict__ row_amax, int64_t positions, int top_k,
+__device__ __forceinline__ void count_segment(const int64_t* top_idx,
+                                              const uint16_t* row_amax, int64_t positions, int top_k,
                                               int experts, Passes passes, int groups, int seg_len, int seg,
                                               uint32_t* h, uint32_t* hm, int32_t* __restrict__ seg_count,
                                               uint32_t* __restrict__ seg_max) {
@@ -103,7 +103,7 @@ __device__ __forceinline__ void count_segment(const int64_t* __restrict__ top_id
   }
 }
 
-__global__ void dispatch_count_kernel(const int64_t* __restrict__ top_idx, const uint16_t* __restrict__ row_amax,
+__global__ void dispatch_count_kernel(const int64_t* top_idx, const uint16_t* row_amax,
                                       int64_t positions, int top_k, int experts, Passes passes, int groups,
                                       int seg_len, int segments, int32_t* __restrict__ seg_count,
                                       uint32_t* __restrict__ seg_max) {
@@ -155,7 +155,7 @@ __device__ int block_exclusive_scan(int v, int* s_warp, int* total) {
 // 2. scan (single CTA of 1024 threads; experts <= 1024)
 // ---------------------------------------------------------------------------
 __device__ void scan_segments(
-    int32_t* __restrict__ seg_count, const uint32_t* __restrict__ seg_max, int segments, int experts,
+    int32_t* __restrict__ seg_count, const uint32_t* seg_max, int segments, int experts,
     int64_t positions, int align, int32_t* __restrict__ offsets, int32_t* __restrict__ csr,
     int32_t* __restrict__ pcsr, TileEntry* __restrict__ tiles, int max_tiles, int32_t* __restrict__ num_tiles,
     float* __restrict__ act_global, uint32_t* __restrict__ act_amax_bits) {
@@ -280,7 +280,7 @@ __device__ void scan_segments(
 }
 
 __global__ void __launch_bounds__(1024) dispatch_scan_kernel(
-    int32_t* __restrict__ seg_count, const uint32_t* __restrict__ seg_max, int segments, int experts,
+    int32_t* __restrict__ seg_count, const uint32_t* seg_max, int segments, int experts,
     int64_t positions, int align, int32_t* __restrict__ offsets, int32_t* __restrict__ csr,
     int32_t* __restrict__ pcsr, TileEntry* __restrict__ tiles, int max_tiles, int32_t* __restrict__ num_tiles,
     float* __restrict__ act_global, uint32_t* __restrict__ act_amax_bits) {
@@ -297,8 +297,8 @@ __global__ void __launch_bounds__(1024) dispatch_scan_kernel(
 // tiles and 256-row pairs are laid out as by the dispatch, with v as the
 // tile's expert. One CTA of 1024 threads, segments <= 1024.
 // ---------------------------------------------------------------------------
-__global__ void __launch_bounds__(1024) segment_tiles_kernel(const int32_t* __restrict__ counts,
-                                                             const int32_t* __restrict__ starts, int segments,
+__global__ void __launch_bounds__(1024) segment_tiles_kernel(const int32_t* counts,
+                                                             const int32_t* starts, int segments,
                                                              TileEntry* __restrict__ tiles, int max_tiles,
                                                              int32_t* __restrict__ num_tiles) {
   pdl_wait();  // the previous kernel of the stream has completed
@@ -354,8 +354,8 @@ int run_segment_tiles(const int32_t* counts, const int32_t* starts, int segments
 // ---------------------------------------------------------------------------
 // One warp's segment: its routed positions in order into their rows, from
 // the warp's cursor row (cur[g] = csr[g] + the segment's start in group g).
-__device__ __forceinline__ void scatter_segment(const int64_t* __restrict__ top_idx,
-                                                const uint16_t* __restrict__ gate, int64_t positions, int top_k,
+__device__ __forceinline__ void scatter_segment(const int64_t* top_idx,
+                                                const uint16_t* gate, int64_t positions, int top_k,
                                                 int experts, Passes passes, int seg_len, int seg, int32_t* cur,
                                                 int64_t* __restrict__ order, int64_t* __restrict__ inverse,
                                                 int64_t* __restrict__ tokens, int32_t* __restrict__ tokens32,
@@ -398,10 +398,10 @@ __device__ __forceinline__ void scatter_segment(const int64_t* __restrict__ top_
   }
 }
 
-__global__ void dispatch_scatter_kernel(const int64_t* __restrict__ top_idx, const uint16_t* __restrict__ gate,
+__global__ void dispatch_scatter_kernel(const int64_t* top_idx, const uint16_t* gate,
                                         int64_t positions, int top_k, int experts, Passes passes, int groups,
                                         int seg_len, int segments,
-                                        const int32_t* __restrict__ seg_start, const int32_t* __restrict__ csr,
+                                        const int32_t* seg_start, const int32_t* csr,
                                         int64_t* __restrict__ order, int64_t* __restrict__ inverse,
                                         int64_t* __restrict__ tokens, int32_t* __restrict__ tokens32,
                                         uint16_t* __restrict__ sorted_gate) {
@@ -428,7 +428,7 @@ constexpr int kFusedWarps = 32;
 constexpr int kFusedMaxGroups = 256;
 
 __global__ void __launch_bounds__(1024) dispatch_fused_kernel(
-    const int64_t* __restrict__ top_idx, const uint16_t* __restrict__ gate, const uint16_t* __restrict__ row_amax,
+    const int64_t* top_idx, const uint16_t* gate, const uint16_t* row_amax,
     int64_t positions, int top_k, int experts, Passes passes, int groups, int seg_len, int segments,
     int32_t* __restrict__ seg_count, uint32_t* __restrict__ seg_max, int32_t* __restrict__ offsets,
     int32_t* __restrict__ csr, int32_t* __restrict__ pcsr, TileEntry* __restrict__ tiles, int max_tiles,

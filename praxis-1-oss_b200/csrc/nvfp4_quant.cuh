@@ -111,7 +111,7 @@ __device__ __forceinline__ void unpack16_bf16(const uint32_t (&w)[8], float (&v)
 // The same for 16 bf16 values read from global memory (32 bytes, aligned).
 __device__ __forceinline__ void load16_bf16_fast(const uint16_t* src, float (&v)[16], float& amax, bool& has_nan) {
   const uint4* s = reinterpret_cast<const uint4*>(src);
-  const uint4 a = __ldg(s), b = __ldg(s + 1);
+  const uint4 a = s[0], b = s[1];
   const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
   unpack16_bf16(w, v, amax, has_nan);
 }

@@ -89,8 +89,8 @@ constexpr int kGatherWarps = 8;
 
 // Zero the padding rows of partly filled tiles (the reference allocates
 // these buffers with zeros, praxis/kernels/nvfp4.py:227-231); one CTA per tile.
-__device__ __forceinline__ void gather_zero_padding(int m, int k_dim, const TileEntry* __restrict__ tiles,
-                                                    const int32_t* __restrict__ num_tiles, uint8_t* __restrict__ q,
+__device__ __forceinline__ void gather_zero_padding(int m, int k_dim, const TileEntry* tiles,
+                                                    const int32_t* num_tiles, uint8_t* __restrict__ q,
                                                     uint8_t* __restrict__ sf, bool rep) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int kb = k_dim / 16;
@@ -123,10 +123,10 @@ __device__ __forceinline__ void gather_zero_padding(int m, int k_dim, const Tile
 // rows of partly filled tiles, one tile each.
 template <int K>
 __global__ void __launch_bounds__(256) quantize_gather_kernel(
-    const uint16_t* __restrict__ x, int64_t tokens, int k_dim, const int64_t* __restrict__ top_idx,
-    const int64_t* __restrict__ inverse, const int32_t* __restrict__ csr, const int32_t* __restrict__ pcsr,
-    const float* __restrict__ globals, const uint32_t* __restrict__ amax_bits, int experts, Passes passes,
-    const TileEntry* __restrict__ tiles, const int32_t* __restrict__ num_tiles, int token_blocks,
+    const uint16_t* x, int64_t tokens, int k_dim, const int64_t* top_idx,
+    const int64_t* inverse, const int32_t* csr, const int32_t* pcsr,
+    const float* globals, const uint32_t* amax_bits, int experts, Passes passes,
+    const TileEntry* tiles, const int32_t* num_tiles, int token_blocks,
     uint8_t* __restrict__ q, uint8_t* __restrict__ sf, bool rep) {
   pdl_wait();  // the previous kernel of the stream has completed
   pdl_trigger();
@@ -142,8 +142,8 @@ __global__ void __launch_bounds__(256) quantize_gather_kernel(
   const uint4* xr = reinterpret_cast<const uint4*>(x + t * k_dim);
   uint4 na = make_uint4(0, 0, 0, 0), nb = na;
   if (lane < kb) {
-    na = __ldg(xr + 2 * lane);
-    nb = __ldg(xr + 2 * lane + 1);
+    na = xr[2 * lane];
+    nb = xr[2 * lane + 1];
   }
   int64_t my_dest = 0;
   float my_g = 1.0f;
@@ -175,8 +175,8 @@ __global__ void __launch_bounds__(256) quantize_gather_kernel(
     const uint32_t w[8] = {na.x, na.y, na.z, na.w, nb.x, nb.y, nb.z, nb.w};
     const int jn = j0 + 32 + lane;
     if (jn < kb) {
-      na = __ldg(xr + 2 * jn);
-      nb = __ldg(xr + 2 * jn + 1);
+      na = xr[2 * jn];
+      nb = xr[2 * jn + 1];
     }
     const int j = j0 + lane;
     const bool active = j < kb;
@@ -203,8 +203,8 @@ __global__ void __launch_bounds__(256) quantize_gather_kernel(
 // Row quantize of the hidden activations (one warp per padded row of a tile)
 // ---------------------------------------------------------------------------
 __global__ void __launch_bounds__(256) quantize_rows_kernel(
-    const uint16_t* __restrict__ x, int k_dim, const TileEntry* __restrict__ tiles,
-    const int32_t* __restrict__ num_tiles, const float* __restrict__ globals, const uint32_t* __restrict__ amax_bits,
+    const uint16_t* x, int k_dim, const TileEntry* tiles,
+    const int32_t* num_tiles, const float* globals, const uint32_t* amax_bits,
     uint8_t* __restrict__ q, uint8_t* __restrict__ sf, bool rep) {
   pdl_wait();  // the previous kernel of the stream has completed
   pdl_trigger();
@@ -309,7 +309,7 @@ __global__ void interleave_gate_up_kernel(const uint8_t* __restrict__ q, const u
 // Compact -> replicated scales: one thread per 16-byte chunk (one row of 32
 // within the atom: 4 quadrants x 4 scales), written to the four copies.
 // ---------------------------------------------------------------------------
-__global__ void replicate_scales_kernel(const uint4* __restrict__ sf, int64_t chunks, int kb, int group_rows,
+__global__ void replicate_scales_kernel(const uint4* sf, int64_t chunks, int kb, int group_rows,
                                         uint4* __restrict__ out) {
   pdl_wait();  // the previous kernel of the stream has completed
   pdl_trigger();

@@ -229,7 +229,7 @@ __device__ __forceinline__ uint64_t shfl_xor_u64(uint64_t v, int o) {
 // P = experts per lane (experts <= 32 * P), K = top_k (the selection, tie
 // and order loops unroll to K entries).
 template <int P, int K>
-__global__ void __launch_bounds__(256) route_kernel(const float* __restrict__ logits, const float* __restrict__ bias,
+__global__ void __launch_bounds__(256) route_kernel(const float* logits, const float* bias,
                                                     int64_t tokens, int experts, int activation,
                                                     int64_t* __restrict__ top_idx, uint16_t* __restrict__ gate) {
   pdl_wait();  // the previous kernel of the stream has completed

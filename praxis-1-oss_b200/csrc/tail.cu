@@ -55,10 +55,10 @@ __device__ __forceinline__ int64_t mod_row(int64_t row, const int64_t* g) {
 // modulation between them.
 template <int KMAX, bool NORM, bool MOD>
 __global__ void __launch_bounds__(256) combine_tail_kernel(
-    const uint16_t* __restrict__ rows, int cols, const int64_t* __restrict__ inverse,
-    const int64_t* __restrict__ top_idx, const uint16_t* __restrict__ gate, const int32_t* __restrict__ csr,
-    const int32_t* __restrict__ pcsr, const float* __restrict__ h_global, const uint32_t* __restrict__ h_amax,
-    const float* __restrict__ w_global, int rows_rescaled, float scaling, const uint16_t* __restrict__ shared,
+    const uint16_t* rows, int cols, const int64_t* inverse,
+    const int64_t* top_idx, const uint16_t* gate, const int32_t* csr,
+    const int32_t* pcsr, const float* h_global, const uint32_t* h_amax,
+    const float* w_global, int rows_rescaled, float scaling, const uint16_t* shared,
     TailArgs tail, int64_t tokens, int top_k, int experts, Passes passes) {
   pdl_wait();  // the previous kernel of the stream has completed
   pdl_trigger();

@@ -320,6 +320,20 @@ def test_the_streamed_tails_dispatch_is_complete_before_its_combine_starts():
     assert ffn.index("run_fp8_identity(") < ffn.index("run_fp8_stream_ffn(") < ffn.index("run_combine_tail(")
 
 
+def test_no_overlapping_kernel_reads_its_inputs_as_read_only_data():
+    """The same for every kernel that waits for its predecessor, and for the device
+    functions beside them."""
+    for path in sorted(CSRC.glob("*.cu*")):
+        text = code(path.name)
+        if "pdl_wait" not in text and path.suffix == ".cu":
+            continue
+        for name, params, body in re.findall(r"\b(\w+)\(([^()]*)\)\s*\{(.*?)\n}\n", text, re.S):
+            if name + "<<<" in text:
+                continue  # launched behind its predecessor's end
+            assert not re.search(r"const \w+\* __restrict__", params), (path.name, name)
+            assert set(re.findall(r"__ldg\(\s*(\w+)", body)) <= {"ws"}, (path.name, name)
+
+
 # -- workspaces --------------------------------------------------------------------
 
 def ffn_workspace(tokens, top_k, experts, dim, hidden):

@@ -445,11 +445,13 @@ int praxis_b200_fp8_linear(const void* x, int64_t rows, int32_t k, int64_t ldx, 
 
 /* A SwiGLU feed-forward on block-scaled weights, dense (a shared expert) or
  * routed (top_k > 0): h = silu(x G^T) * (x U^T) in fp32, quantized per
- * 128 columns as above, y = h D^T rounded to bf16. gate_up_q [E, 2F, C] holds
- * G then U, gate_up_scale [E, 2F/128, C/128], down_q [E, C, F], down_scale
- * [E, C/128, F/128]; dense: E = 1. Routed: E <= 1024, k <= 8, and the combine
- * of praxis_b200_moe_forward (out[t] = bf16(sum of gate * scaling * y), then
- * bf16(out + shared)). Dense: out = y; gate, scaling and shared are not used.
+ * 128 columns as above, y = h D^T. gate_up_q [E, 2F, C] holds G then U,
+ * gate_up_scale [E, 2F/128, C/128], down_q [E, C, F], down_scale
+ * [E, C/128, F/128]; dense: E = 1. Routed: E <= 1024, k <= 8, out[t] =
+ * bf16(sum of gate * scaling * y), summed in fp32, then bf16(out + shared).
+ * More than 8 + E / 8 routed slots: each y is rounded to bf16 before that sum
+ * (as by praxis_b200_moe_forward); fewer, which are streamed: y stays fp32.
+ * Dense: out = bf16(y); gate, scaling and shared are not used.
  * C and F multiples of 128, buffers 16-byte, the workspace 32-byte aligned. */
 typedef struct praxis_b200_fp8_ffn_args {
   const void* x;              /* [T, C] bf16 */

@@ -136,6 +136,7 @@ __global__ void __launch_bounds__(kFp8SlotThreads) fp8_slots_kernel(
 // shuffles. Scales are stored block-major, scale[b * scale_ld + row]: the GEMM
 // epilogue reads one block's scales of 32 consecutive rows at once. With
 // `top_idx` the row goes to the rows of the token's routed slots, quantized once.
+// Six CTAs per SM hold the kernel at 40 registers (11 of them spilled).
 struct Fp8Rows {
   const int64_t* top_idx;  // [rows, top_k]; nullptr: row r goes to row r
   const int64_t* inverse;
@@ -323,7 +324,9 @@ struct Fp8Shape {
   static constexpr int COLS = 4 * BN / EPI_WARPS;  // columns per epilogue thread
   // Registers: 12 warps launch with 168 each (64512 in all); the first four
   // give some back, and the epilogue's 128 sums and two 16-column loads in
-  // flight fit without spilling. 8 warps (BN = 64) have enough as they are.
+  // flight fit (ptxas spills 60 bytes of the plain instance's other values, 20 of
+  // the SwiGLU one's; of those with few rows 104 and none). 8 warps (BN = 64)
+  // have enough as they are.
   static constexpr int EPI_WARP0 = 4;
   static constexpr int THREADS = 32 * (EPI_WARP0 + EPI_WARPS);
   static constexpr bool SPLIT_REGS = EPI_WARPS == 8;

@@ -422,7 +422,7 @@ __global__ void __launch_bounds__(256) route_kernel(const float* logits, const f
 // warp's largest head of a list (redux.sync), the lowest lane that has it, and
 // one shift of that lane's list. Which expert a pick was, and its score, are
 // found for all picks at once at the end. Bound by the instructions it issues,
-// about 770 per token of 256 experts (16384 tokens 15.5 us; 22 with a scan of
+// about 770 per token of 256 experts (16384 tokens 14.3 us; 22 with a scan of
 // the owner's experts per pick). The scores are those of route_kernel's sigmoid;
 // the softmax sum is held in 64 bits and rounded once, so that its order moves
 // no comparison.

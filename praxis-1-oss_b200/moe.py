@@ -2,11 +2,12 @@
 the router and the routed experts on this library's sm_100a kernels.
 
 Constructor, state-dict keys (``router.weight``, ``expert_bias``,
-``routed.*`` packed NVFP4 buffers, ``shared.gate_up``, ``shared.down``) and the
+``routed.*`` packed buffers, ``shared.gate_up``, ``shared.down``) and the
 forward contract follow the reference module; the routed bank is a
-``B200NVFP4RoutedExperts``. The shared expert stays a torch bf16 SwiGLU (the
-reference's ``SharedExpert``, praxis/layers.py:1033-1089), added after the
-routed sum is rounded to bf16.
+``B200NVFP4RoutedExperts``, or a ``B200FP8RoutedExperts`` for block-scaled FP8
+weights. The shared expert is a torch bf16 SwiGLU (the reference's
+``SharedExpert``, praxis/layers.py:1033-1089) or a ``FP8SharedExpert``, added
+after the routed sum is rounded to bf16.
 """
 
 from __future__ import annotations

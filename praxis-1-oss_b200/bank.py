@@ -339,7 +339,11 @@ def routed_forward_tail(bank: B200NVFP4RoutedExperts, x: Tensor, top_idx: Tensor
     ``tail.residual``, then, when ``tail.norm_weight`` is set, the next block's
     RMSNorm (with its modulation when ``tail.mod`` is set). Returns ``(new
     residual, normed rows or None)`` with the eager bits; the routed output
-    itself is never stored. Each dispatch chunk fuses its own rows."""
+    itself is never stored. Each dispatch chunk fuses its own rows. A bank that
+    has a ``routed_forward_tail`` of its own (``B200FP8RoutedExperts``) runs it."""
+    if hasattr(bank, "routed_forward_tail"):
+        return bank.routed_forward_tail(x, top_idx, gate, scaling=scaling, chunk_size=chunk_size, tail=tail,
+                                        shared=shared)
     bank._check(x, top_idx, gate, scaling, chunk_size)
     r = tail.residual
     if r.shape != x.shape or r.dtype != torch.bfloat16 or not r.is_contiguous() or r.device != x.device:

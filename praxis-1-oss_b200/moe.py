@@ -13,7 +13,6 @@ after the routed sum is rounded to bf16.
 from __future__ import annotations
 
 import os
-from functools import partial
 
 import torch
 import torch.nn.functional as F
@@ -248,10 +247,8 @@ class B200MoEFeedForward(nn.Module):
                                  mod_geom=None if geom is None else tuple(int(v) for v in geom))
         chunk = self.dispatch_chunk_size or max(1, x_flat.shape[0])
         with _Range("routed"):
-            run = (self.routed.routed_forward_tail if isinstance(self.routed, B200FP8RoutedExperts)
-                   else partial(routed_forward_tail, self.routed))
-            xo, h = run(x_flat, top_idx, gate, scaling=self.routed_scaling_factor, chunk_size=chunk, tail=tail,
-                        shared=y_shared)
+            xo, h = routed_forward_tail(self.routed, x_flat, top_idx, gate, scaling=self.routed_scaling_factor,
+                                        chunk_size=chunk, tail=tail, shared=y_shared)
         return xo.reshape(shape), None if h is None else h.reshape(shape)
 
     @torch.no_grad()

@@ -254,6 +254,23 @@ def test_bank_checks_the_whole_call_before_it_is_cut_in_chunks(monkeypatch, kind
     assert not called
 
 
+def test_the_tail_function_takes_either_bank(monkeypatch):
+    """``praxis_b200.routed_forward_tail`` runs an FP8 bank's own tail."""
+    rows = []
+
+    def fake(x, *args, tail, tail_out, **kwargs):
+        rows.append(x.shape[0])
+        tail_out[0].copy_(tail.residual)
+
+    monkeypatch.setattr(pkg().ops, "fp8_moe_forward", fake)
+    bank = pkg().B200FP8RoutedExperts.from_packed(packed())
+    x, residual = torch.ones(5, 128, dtype=BF16), torch.randn(5, 128).to(BF16)
+    new, normed = pkg().routed_forward_tail(
+        bank, x, torch.zeros(5, 2, dtype=torch.int64), torch.ones(5, 2, dtype=BF16), scaling=1.0, chunk_size=2,
+        tail=pkg().ops.Tail(residual), shared=x)
+    assert rows == [2, 2, 1] and torch.equal(new, residual) and normed is None
+
+
 def test_module_takes_groups_and_formats():
     M = pkg().B200MoEFeedForward
     m = M(128, 128, 16, 4, router_groups=4, router_top_groups=2)

@@ -853,8 +853,8 @@ int praxis_b200_fp8_ffn(const praxis_b200_fp8_ffn_args* a) {
     uint16_t* gate = reinterpret_cast<uint16_t*>(ws + L.stream_gate);
     int32_t* csr = reinterpret_cast<int32_t*>(ws + L.stream_csr);
     int32_t* pcsr = reinterpret_cast<int32_t*>(ws + L.stream_pcsr);
-    // before the products: the combine reads its dispatch as read-only data, so
-    // the kernel that writes it has to be over when the combine starts
+    // before the products, so that the combine's dispatch is complete when the
+    // combine starts: its direct predecessor writes nothing but the rows
     if (a->tail) {
       rc = run_fp8_identity((int)a->tokens, inverse, top_idx, gate, csr, pcsr, s);
       if (rc) return rc;

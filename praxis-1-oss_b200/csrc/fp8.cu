@@ -431,9 +431,9 @@ constexpr int kFp8FewRows = 32;
 // serves both columns: 1 / (d0 d1) times the other denominator, 1 <= d <= 2.
 // Relative error: about 2^-21 of the approximations and products plus |g| 2^-24
 // of the rounded exponent (2^-18 for a gate of -40), against the 2^-4 of the
-// rounding to E4M3 that follows. exp(-|g|) below 2^-126 is 0: a gate below -87.3 gives 0 in place
-// of at most 1.1e-36 |u|. As the quotient has it, NaN stays NaN and a gate of
-// -inf gives NaN.
+// rounding to E4M3 that follows. exp(-|g|) below 2^-126 is 0: a gate below
+// -87.3 gives 0 in place of at most 1.1e-36 |u|. As the quotient has it, NaN
+// stays NaN and a gate of -inf gives NaN.
 __device__ __forceinline__ void swiglu_pair_f32(float& g0, float& g1, float u0, float u1) {
   float s0, s1, r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(s0) : "f"(-1.4426950408889634f * fabsf(g0)));
